@@ -60,6 +60,11 @@ class Status(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("code", "cuda_error", "where", "layer", "block", "expected", "seen")]
 
 
+class Kv4Seqs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_pool", "d_table", "d_start", "d_cached", "d_status")] + \
+               [(n, ctypes.c_int32) for n in ("cached", "n_pages", "n_kv_head", "head_dim", "n_seq", "table_ld", "n_tokens", "device")]
+
+
 # every symbol include/flint_b200.h declares, with its prototype
 _PROTOS = {
     "fb_query": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(Caps)]),
@@ -105,6 +110,16 @@ _PROTOS = {
                                      ctypes.c_void_p, ctypes.c_void_p]),
     "fb_kv_move": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32),
                                   ctypes.c_int32, ctypes.c_void_p]),
+    "fb_kv4_page_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32]),
+    "fb_kv4_append": (ctypes.c_int, [ctypes.POINTER(Kv4Seqs), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                     ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                     ctypes.c_void_p]),
+    "fb_kv4_attend": (ctypes.c_int, [ctypes.POINTER(Kv4Seqs), ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                     ctypes.c_void_p, ctypes.c_int32, ctypes.c_float, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "fb_kv4_read": (ctypes.c_int, [ctypes.POINTER(Kv4Seqs), ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "fb_kv4_compact": (ctypes.c_int, [ctypes.POINTER(Kv4Seqs), ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p]),
+    "fb_kv4_move": (ctypes.c_int, [ctypes.POINTER(Kv4Seqs), ctypes.c_int32, ctypes.c_int64, ctypes.POINTER(ctypes.c_int32),
+                                   ctypes.POINTER(ctypes.c_int32), ctypes.c_int32, ctypes.c_void_p]),
 }
 EXPORTED_SYMBOLS = tuple(_PROTOS)
 

@@ -46,6 +46,13 @@ __device__ __forceinline__ float bfhi(uint32_t p) { return __uint_as_float(p & 0
 __device__ __forceinline__ uint16_t f2bf(float f) { return __bfloat16_as_ushort(__float2bfloat16_rn(f)); }
 __device__ __forceinline__ float rbf(float f) { return bf2f(f2bf(f)); }   // round an fp32 value to bf16 precision
 
+// the power of two that brings a bound `a` on some magnitudes into [2^14, 2^15), and its inverse (both finite for every a >= 0)
+__device__ __forceinline__ float2 pow2_for(float a) {
+  uint32_t mf = 268u - ((__float_as_uint(a) >> 23) & 255u);
+  mf = mf > 253u ? 253u : (mf < 24u ? 24u : mf);
+  return make_float2(__uint_as_float(mf << 23), __uint_as_float((254u - mf) << 23));
+}
+
 __device__ __forceinline__ unsigned long long globaltimer_ns() {
   unsigned long long t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));

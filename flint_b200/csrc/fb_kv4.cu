@@ -1,0 +1,181 @@
+// extern "C" entry points of the 4-bit paged K/V cache: append, attention, read-back, moves.
+// No torch types, no CPU fallback: a failed CUDA call or an unsupported shape is an error code.
+#include <string.h>
+
+#include "../../include/flint_b200.h"
+#include "fb_ctx.hpp"
+#include "fb_kv4.cuh"
+
+using namespace fb;
+
+namespace {
+
+int device_sms(int dev) {
+  static int sms[64] = {};
+  if (dev < 0 || dev >= 64) return 0;
+  if (!sms[dev] && cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  return sms[dev];
+}
+
+// FB_OK and the kernels' view of the sequences, or why not
+int take_seqs(const fb_kv4_seqs* s, int rows_of_tokens, Kv4Seqs& S) {
+  if (!s || !s->d_pool || !s->d_table || !s->d_status) return FB_ERR_ARG;
+  if (((uintptr_t)s->d_pool & 15) || ((uintptr_t)s->d_table & 3) || ((uintptr_t)s->d_start & 3) || ((uintptr_t)s->d_cached & 3) || ((uintptr_t)s->d_status & 3))
+    return FB_ERR_ARG;
+  if (s->head_dim != 64 && s->head_dim != 80 && s->head_dim != 128) return FB_ERR_SHAPE;
+  if (s->n_kv_head < 1 || s->n_kv_head > 65535 || s->n_pages < 1 || s->table_ld < 1 || s->n_seq < 0 || s->n_tokens < 0) return FB_ERR_ARG;
+  if (s->table_ld > 0x7fffffff / kPage) return FB_ERR_RANGE;
+  if (rows_of_tokens && s->n_seq > 1 && !s->d_start) return FB_ERR_ARG;
+  if (!s->d_cached && (s->cached < 0 || (!s->d_start && (int64_t)s->cached + s->n_tokens > (int64_t)s->table_ld * kPage))) return FB_ERR_RANGE;
+  S = Kv4Seqs{(uint8_t*)s->d_pool, s->d_table, s->d_start, s->d_cached, s->cached, s->n_pages, s->n_kv_head, s->n_seq, s->table_ld, s->n_tokens, (DevStatus*)s->d_status};
+  return FB_OK;
+}
+int done(cudaError_t e) { return e == cudaSuccess ? FB_OK : FB_ERR_CUDA; }
+
+// rows of 16-bit numbers that are read 16 bytes at a time
+bool rows_ok(const void* p, int64_t ld, int64_t width) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld >= width; }
+
+template <int HD, int NQ, int W>
+cudaError_t launch_few(Kv4Attend p, int max_len, int sms, cudaStream_t st) {
+  using F = Kv4Few<HD, NQ, W>;
+  static bool configured[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  auto k = kv4_attn_few<HD, NQ, W>;
+  if (!configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, F::TOTAL);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  p.groups = (int)(((int64_t)p.max_new * p.R + F::ROWS - 1) / F::ROWS);
+  const int64_t items = (int64_t)p.S.n_seq * p.groups, units = ((int64_t)max_len + F::U - 1) / F::U;
+  int ns = 1;
+  while (ns < 16 && items * p.S.nkv * ns * 2 <= sms && units >= (int64_t)ns * 2 * W) ns *= 2;
+  p.nsplit = ns;
+  if (items * ns > 0x7fffffff) return cudaErrorInvalidValue;
+  return launch_pdl_cluster(k, dim3((unsigned)(items * ns), (unsigned)p.S.nkv), dim3(W * 32), (size_t)F::TOTAL, st, (unsigned)ns, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fb_kv4_page_bytes(int32_t n_kv_head, int32_t head_dim) {
+  if (n_kv_head < 1 || (head_dim != 64 && head_dim != 80 && head_dim != 128)) return 0;
+  return (size_t)n_kv_head * (kPage / 16) * (16 * (size_t)head_dim + 128);
+}
+
+int fb_kv4_append(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, const void* d_k, int64_t k_ld, const void* d_v, int64_t v_ld, int32_t n_head,
+                  const int32_t* d_depth, const uint64_t* d_freq, void* d_q_out, int64_t qo_ld, void* stream) {
+  Kv4Append p;
+  const int rc = take_seqs(s, 1, p.S);
+  if (rc != FB_OK) return rc;
+  if (s->n_tokens == 0 || s->n_seq == 0) return FB_OK;
+  const int64_t hd = s->head_dim, kw = hd * s->n_kv_head, qw = hd * n_head;
+  if (!d_k || !d_v || !rows_ok(d_k, k_ld, kw) || !rows_ok(d_v, v_ld, kw) || ((uintptr_t)d_freq & 7) || ((uintptr_t)d_depth & 3)) return FB_ERR_ARG;
+  if (d_q && (!d_q_out || n_head < 1 || !rows_ok(d_q, q_ld, qw) || !rows_ok(d_q_out, qo_ld, qw))) return FB_ERR_ARG;
+  DeviceGuard g(s->device);
+  const int sms = device_sms(s->device);
+  if (!g.ok || !sms) return FB_ERR_CUDA;
+  p.q = (const uint16_t*)d_q; p.k = (const uint16_t*)d_k; p.v = (const uint16_t*)d_v; p.q_out = (uint16_t*)d_q_out;
+  p.q_ld = q_ld; p.k_ld = k_ld; p.v_ld = v_ld; p.qo_ld = qo_ld;
+  p.depth = d_depth; p.freq = (const unsigned long long*)d_freq; p.nh = n_head;
+  const int groups = ((d_q ? n_head : 0) + 2 * s->n_kv_head + 7) / 8, room = 4 * sms / s->n_tokens;
+  const dim3 grid(s->n_tokens, groups < room ? groups : (room > 1 ? room : 1)), block(256);
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (s->head_dim) {
+    case 64: return done(launch_pdl(kv4_append<64>, grid, block, 0, st, p));
+    case 80: return done(launch_pdl(kv4_append<80>, grid, block, 0, st, p));
+    default: return done(launch_pdl(kv4_append<128>, grid, block, 0, st, p));
+  }
+}
+
+int fb_kv4_read(const fb_kv4_seqs* s, int32_t n_layer, int64_t layer_bytes, float* d_k, float* d_v, void* stream) {
+  Kv4Read p;
+  const int rc = take_seqs(s, 1, p.S);
+  if (rc != FB_OK) return rc;
+  if (n_layer < 1 || n_layer > 65535 || layer_bytes < 0 || layer_bytes % 16 || ((uintptr_t)d_k & 15) || ((uintptr_t)d_v & 15)) return FB_ERR_ARG;
+  if (s->n_tokens == 0 || s->n_seq == 0 || (!d_k && !d_v)) return FB_OK;
+  DeviceGuard g(s->device);
+  if (!g.ok) return FB_ERR_CUDA;
+  p.k = d_k; p.v = d_v; p.layer = (size_t)layer_bytes;
+  const dim3 grid(s->n_tokens, n_layer), block(256);
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (s->head_dim) {
+    case 64: return done(launch_pdl(kv4_read<64>, grid, block, 0, st, p));
+    case 80: return done(launch_pdl(kv4_read<80>, grid, block, 0, st, p));
+    default: return done(launch_pdl(kv4_read<128>, grid, block, 0, st, p));
+  }
+}
+
+static int launch_move(const fb_kv4_seqs* s, const Kv4Move& p, int32_t n_layer, cudaStream_t st) {
+  const dim3 grid(s->n_kv_head, n_layer), block(128);
+  switch (s->head_dim) {
+    case 64: return done(launch_pdl(kv4_move<64>, grid, block, 0, st, p));
+    case 80: return done(launch_pdl(kv4_move<80>, grid, block, 0, st, p));
+    default: return done(launch_pdl(kv4_move<128>, grid, block, 0, st, p));
+  }
+}
+
+int fb_kv4_compact(const fb_kv4_seqs* s, int32_t n_layer, int64_t layer_bytes, const int32_t* d_accept, int32_t most, void* stream) {
+  Kv4Move p;
+  memset(&p, 0, sizeof(p));
+  const int rc = take_seqs(s, 0, p.S);
+  if (rc != FB_OK) return rc;
+  if (!d_accept || ((uintptr_t)d_accept & 3) || most < 0 || n_layer < 1 || n_layer > 65535 || layer_bytes < 0 || layer_bytes % 16 || s->d_cached) return FB_ERR_ARG;
+  if (s->cached > s->table_ld * kPage - 1) return FB_ERR_RANGE;
+  DeviceGuard g(s->device);
+  if (!g.ok) return FB_ERR_CUDA;
+  p.layer = (size_t)layer_bytes; p.accept = d_accept; p.pos = s->cached; p.most = most;
+  return launch_move(s, p, n_layer, (cudaStream_t)stream);
+}
+
+int fb_kv4_move(const fb_kv4_seqs* s, int32_t n_layer, int64_t layer_bytes, const int32_t* src, const int32_t* dst, int32_t n, void* stream) {
+  Kv4Move p;
+  memset(&p, 0, sizeof(p));
+  const int rc = take_seqs(s, 0, p.S);
+  if (rc != FB_OK) return rc;
+  if (n < 0 || (n > 0 && (!src || !dst)) || n_layer < 1 || n_layer > 65535 || layer_bytes < 0 || layer_bytes % 16) return FB_ERR_ARG;
+  const int64_t slots = (int64_t)s->table_ld * kPage;
+  for (int i = 0; i < n; i++)
+    if (src[i] < 0 || dst[i] < 0 || src[i] >= slots || dst[i] >= slots) return FB_ERR_RANGE;
+  DeviceGuard g(s->device);
+  if (!g.ok) return FB_ERR_CUDA;
+  p.layer = (size_t)layer_bytes;
+  for (int i0 = 0; i0 < n; i0 += 64) {                           // the moves of a launch travel in its parameters
+    p.n = n - i0 < 64 ? n - i0 : 64;
+    memcpy(p.src, src + i0, p.n * sizeof(int));
+    memcpy(p.dst, dst + i0, p.n * sizeof(int));
+    const int e = launch_move(s, p, n_layer, (cudaStream_t)stream);
+    if (e != FB_OK) return e;
+  }
+  return FB_OK;
+}
+
+int fb_kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n_head, int32_t max_new, int32_t max_len, const uint8_t* d_amask,
+                  int32_t mask_ld, float scale, void* d_out, int64_t o_ld, void* stream) {
+  Kv4Attend p;
+  const int rc = take_seqs(s, 1, p.S);
+  if (rc != FB_OK) return rc;
+  if (s->n_tokens == 0 || s->n_seq == 0) return FB_OK;
+  const int64_t qw = (int64_t)s->head_dim * n_head;
+  if (n_head < 1 || n_head % s->n_kv_head) return FB_ERR_SHAPE;
+  if (!d_q || !d_out || !rows_ok(d_q, q_ld, qw) || !rows_ok(d_out, o_ld, qw) || max_new < 1 || max_len < 1 || (d_amask && mask_ld < 1)) return FB_ERR_ARG;
+  if ((int64_t)s->n_tokens * (n_head / s->n_kv_head) > 0x7fffffff - 256) return FB_ERR_RANGE;      /* rows of a sequence */
+  DeviceGuard g(s->device);
+  const int sms = device_sms(s->device);
+  if (!g.ok || !sms) return FB_ERR_CUDA;
+  p.q = (const uint16_t*)d_q; p.out = (uint16_t*)d_out; p.q_ld = q_ld; p.o_ld = o_ld; p.amask = d_amask; p.mask_ld = mask_ld;
+  p.nh = n_head; p.R = n_head / s->n_kv_head; p.max_new = max_new < s->n_tokens ? max_new : s->n_tokens;
+  p.scale = scale * 1.4426950408889634f; p.spin_limit = 4000000u;
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool one = (int64_t)p.max_new * p.R <= 8;
+  switch (s->head_dim) {
+    case 64: return done(one ? launch_few<64, 1, 16>(p, max_len, sms, st) : launch_few<64, 2, 8>(p, max_len, sms, st));
+    case 80: return done(one ? launch_few<80, 1, 16>(p, max_len, sms, st) : launch_few<80, 2, 8>(p, max_len, sms, st));
+    default: return done(one ? launch_few<128, 1, 16>(p, max_len, sms, st) : launch_few<128, 2, 8>(p, max_len, sms, st));
+  }
+}
+
+}  // extern "C"

@@ -8,13 +8,6 @@ namespace fb {
 
 enum { EPI_QKV = 0, EPI_RESID = 1, EPI_SWIGLU = 2, EPI_LOGITS = 3 };
 
-// the power of two that brings a bound `a` on some magnitudes into [2^14, 2^15), and its inverse (both finite for every a >= 0)
-__device__ __forceinline__ float2 pow2_for(float a) {
-  uint32_t mf = 268u - ((__float_as_uint(a) >> 23) & 255u);
-  mf = mf > 253u ? 253u : (mf < 24u ? 24u : mf);
-  return make_float2(__uint_as_float(mf << 23), __uint_as_float((254u - mf) << 23));
-}
-
 // h[m] = bf16(float(embed[token[m]]) * mult), or a copy of the caller's residual rows
 __global__ void v_embed(const int32_t* tokens, const uint16_t* embed, const uint16_t* h_in, uint16_t* h, int D, int vocab,
                         float mult, int* status_code) {

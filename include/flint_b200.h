@@ -227,6 +227,46 @@ int fb_gemv(const void* d_stream_in, int32_t rows, int32_t k, int32_t has_zeros,
 int fb_gemv_static(const void* d_q, const void* d_s, const void* d_z, int32_t rows, int32_t k, const void* d_x, float* d_y,
                    void* d_status, void* stream);
 
+/* A paged K/V cache of 4 bits a number, for callers that keep many or long sequences (no counterpart in the reference, whose caches are bf16).
+ * A pool of pages of 64 positions; per layer n_pages pages of fb_kv4_page_bytes bytes, 16-byte aligned. A page holds, per kv head, four blocks of 16
+ * positions; a row (position and kv head of K or V) is head_dim nibbles and a bf16 pair (s, z) and stands for (nib - 8) * s + z, with s = bf16((max - min) / 15),
+ * z = bf16(min + 8 s), nib = 8 + clamp(round((x - z) / s), -8, 7), every step in IEEE single precision (s = 0: nib 8). A row with an infinity or a NaN is a row
+ * of NaN. The bytes of a block: flint_b200/csrc/fb_kv4.cuh. head_dim 64, 80 or 128, else FB_ERR_SHAPE.
+ *
+ * fb_kv4_seqs names the sequences of a call and their new tokens:
+ *   d_pool    : one layer (fb_kv4_read / compact / move: the first of n_layer layers, layer_bytes apart)
+ *   d_table   : device int32 [n_seq][table_ld], page of positions 64 i .. 64 i + 63
+ *   d_start   : device int32 [n_seq + 1], tokens d_start[b] .. d_start[b+1] - 1 of the n_tokens are sequence b's; NULL: one sequence has them all. Tokens
+ *               behind the last sequence are left alone
+ *   d_cached  : device int32 [n_seq], positions cached ahead of the new tokens; NULL: `cached` for all. New token i of a sequence has slot cached + i
+ *   d_status  : device int32[8], zeroed once: word 0 becomes FB_ERR_RANGE when a page, a length or a path in device memory cannot be (what it concerns is
+ *               left out, nothing outside the buffers is touched), FB_ERR_TIMEOUT when a bounded wait ran out
+ * The lengths and tables are read when the kernels run: a captured call serves a growing sequence.
+ *
+ *   fb_kv4_append : rotates q (to d_q_out) and k by the angle position * freq and writes k and v into their slots. bf16 rows, tokens *_ld elements apart
+ *                   (multiples of 8, 16-byte aligned). d_freq: device uint64 [head_dim / 2], turns per position in units of 2^-64 (half-split pairs), or NULL: no
+ *                   rotation. d_depth: rotation position of a token behind its sequence's cached ones (tree nodes), or NULL: its place. d_q may be NULL
+ *   fb_kv4_attend : d_out = softmax(scale * q K^T) V over the cached positions and the sequence's own new tokens, which have been appended: causal, or new token j
+ *                   where d_amask[m * mask_ld + j] != 0 (m: token of the call). A token that sees nothing gets zeros. max_new: no sequence has more new
+ *                   tokens (more: FB_ERR_RANGE in d_status); max_len: about the longest sequence, which decides how the work is cut, not what comes out
+ *   fb_kv4_read   : f32 [n_layer][n_tokens][n_kv_head][head_dim], the numbers that the new tokens' rows stand for, bit for bit. d_k or d_v may be NULL
+ *   fb_kv4_compact: fb_kv_compact on sequence 0: slot cached + i takes slot cached + path[i], i = 1 .. len-1, in order; most: entries of the path in d_accept
+ *   fb_kv4_move   : fb_kv_move on sequence 0; src / dst are HOST arrays */
+typedef struct fb_kv4_seqs {
+  void* d_pool;
+  const int32_t *d_table, *d_start, *d_cached;
+  int32_t* d_status;
+  int32_t cached, n_pages, n_kv_head, head_dim, n_seq, table_ld, n_tokens, device;
+} fb_kv4_seqs;
+size_t fb_kv4_page_bytes(int32_t n_kv_head, int32_t head_dim);
+int fb_kv4_append(const fb_kv4_seqs* seqs, const void* d_q, int64_t q_ld, const void* d_k, int64_t k_ld, const void* d_v, int64_t v_ld,
+                  int32_t n_head, const int32_t* d_depth, const uint64_t* d_freq, void* d_q_out, int64_t qo_ld, void* stream);
+int fb_kv4_attend(const fb_kv4_seqs* seqs, const void* d_q, int64_t q_ld, int32_t n_head, int32_t max_new, int32_t max_len,
+                  const uint8_t* d_amask, int32_t mask_ld, float scale, void* d_out, int64_t o_ld, void* stream);
+int fb_kv4_read(const fb_kv4_seqs* seqs, int32_t n_layer, int64_t layer_bytes, float* d_k, float* d_v, void* stream);
+int fb_kv4_compact(const fb_kv4_seqs* seqs, int32_t n_layer, int64_t layer_bytes, const int32_t* d_accept, int32_t most, void* stream);
+int fb_kv4_move(const fb_kv4_seqs* seqs, int32_t n_layer, int64_t layer_bytes, const int32_t* src, const int32_t* dst, int32_t n, void* stream);
+
 /* Tuning / test knobs (no reference counterpart: the reference has no bounded waits and a fixed split).
  *   what 0: iteration limit of every device-side wait (default 4000000); a tiny value makes a launch give up
  *           with FB_ERR_TIMEOUT, which is how the time-out path is tested without hanging a GPU
