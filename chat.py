@@ -50,6 +50,7 @@ def main():
     ap.add_argument("--maxseq", type=int, default=4096)
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--tokens", default="")
+    ap.add_argument("--kv-bits", type=int, default=16, choices=(4, 16), help="bits of a number of the K/V cache")
     ap.add_argument("--selftest", action="store_true")
     a = ap.parse_args()
     torch.set_grad_enabled(False)
@@ -57,10 +58,10 @@ def main():
         from flint_b200.checkpoint import load_hf_checkpoint
         print(f"loading + int4-packing {a.checkpoint} ...", flush=True)
         cfg, packed = load_hf_checkpoint(a.checkpoint, device="cuda")
-        model = Transformer(cfg).load_packed(packed)
+        model = Transformer(cfg, a.kv_bits).load_packed(packed)
     else:
         print(f"building seeded synthetic {a.config} (int4 g128) ...", flush=True)
-        model = Transformer.from_name(a.config).load_synthetic(seed=a.seed)
+        model = Transformer.from_name(a.config, a.kv_bits).load_synthetic(seed=a.seed)
     model.config.block_size = a.maxseq
     cfg: ModelArgs = model.config
     kw = dict(temperature=a.temp, top_k=(a.topk or None), seed=a.seed)

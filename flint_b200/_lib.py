@@ -110,6 +110,7 @@ _PROTOS = {
                                      ctypes.c_void_p, ctypes.c_void_p]),
     "fb_kv_move": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32),
                                   ctypes.c_int32, ctypes.c_void_p]),
+    "fb_bind_kv4": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv4Seqs), ctypes.c_int64, ctypes.c_void_p]),
     "fb_kv4_page_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32]),
     "fb_kv4_append": (ctypes.c_int, [ctypes.POINTER(Kv4Seqs), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
                                      ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,

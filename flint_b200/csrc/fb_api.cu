@@ -452,19 +452,43 @@ int fb_bind_kv(fb_ctx* c, void* d_k, void* d_v, int32_t max_seq) {
   CUtensorMap maps[2];
   FB_CUDA(c, make_kv_maps(c, d_k, d_v, max_seq, maps));        // refused: the context keeps the cache that it had, or none
   c->kc = d_k; c->vc = d_v; c->max_seq = max_seq; c->kmap = maps[0]; c->vmap = maps[1];
+  c->kv4_bound = false;
+  return FB_OK;
+}
+
+int fb_bind_kv4(fb_ctx* c, const fb_kv4_seqs* s, int64_t layer_bytes, const uint64_t* d_freq) {
+  if (!c || !s || !s->d_pool || !s->d_table || !d_freq || ((uintptr_t)s->d_pool & 15) || ((uintptr_t)s->d_table & 3) || ((uintptr_t)d_freq & 7)) return FB_ERR_ARG;
+  if (c->tp_size > 1) return FB_ERR_STATE;                     // a tensor-parallel rank has no M-token pass
+  const fb_model_desc& d = c->d;
+  if (s->head_dim != d.head_dim || s->n_kv_head != d.n_kv_head || !fb_kv4_page_bytes(d.n_kv_head, d.head_dim)) return FB_ERR_SHAPE;
+  if (s->n_pages < 1 || s->table_ld < 1 || s->n_seq != 1 || s->device != c->device || layer_bytes % 16 ||
+      layer_bytes < (int64_t)fb_kv4_page_bytes(d.n_kv_head, d.head_dim) * s->n_pages)
+    return FB_ERR_ARG;
+  if (s->table_ld > 0x7fffffff / 64) return FB_ERR_RANGE;
+  DeviceGuard g(c->device);
+  if (!c->kv4_new) FB_CUDA(c, dmalloc(&c->kv4_new, (size_t)2 * kPromptRows * d.n_kv_head * d.head_dim * 2));
+  if (!c->kv4_logits) FB_CUDA(c, dmalloc(&c->kv4_logits, (size_t)d.vocab * 4));
+  if (!c->kv4_token) FB_CUDA(c, dmalloc(&c->kv4_token, 4));
+  c->kv4 = *s;
+  c->kv4.d_start = c->kv4.d_cached = nullptr;
+  c->kv4.d_status = (int32_t*)c->status;
+  c->kv4_layer = layer_bytes; c->kv4_freq = d_freq;
+  c->max_seq = s->table_ld * 64;
+  c->kv4_bound = true;
   return FB_OK;
 }
 
 int fb_decode(fb_ctx* c, int32_t token, const int32_t* d_token, void* d_h, int32_t pos, float* d_logits, int32_t* d_next,
               void* stream) {
   if (!c) return FB_ERR_ARG;
-  if (!c->weights_bound || !c->kc) return FB_ERR_STATE;
+  if (!c->weights_bound || !has_kv(c)) return FB_ERR_STATE;
   const fb_model_desc& d = c->d;
   if (pos < 0 || pos >= c->max_seq) return FB_ERR_RANGE;
   if (!d_token && !d_h && (token < 0 || (c->tp_size == 1 && token >= d.vocab))) return FB_ERR_RANGE;
   if (!d_h && !c->embed) return FB_ERR_STATE;
   if (d_h && ((uintptr_t)d_h & 1)) return FB_ERR_ARG;
   DeviceGuard g(c->device);
+  if (c->kv4_bound) return pass_decode(c, token, d_token, d_h, pos, d_logits, d_next, (cudaStream_t)stream);
   Decode2Params Q;
   memset(&Q, 0, sizeof(Q));
   Q.w_qkv = c->w_qkv; Q.w_o = c->w_o; Q.w_gu = c->w_gu; Q.w_d = c->w_d; Q.w_lm = c->w_lm;
@@ -544,8 +568,9 @@ int fb_tp_connect_local(fb_ctx* c, fb_ctx* const* ranks, int32_t n) {
 }
 
 int fb_kv_move(fb_ctx* c, const int32_t* src, const int32_t* dst, int32_t n, void* stream) {
-  if (!c || !c->kc || (n > 0 && (!src || !dst))) return FB_ERR_ARG;
+  if (!c || !has_kv(c) || (n > 0 && (!src || !dst))) return FB_ERR_ARG;
   const fb_model_desc& d = c->d;
+  if (c->kv4_bound) return fb_kv4_move(&c->kv4, d.n_layer, c->kv4_layer, src, dst, n, stream);
   DeviceGuard g(c->device);
   const size_t row = (size_t)d.n_kv_head * d.head_dim * 2, layer = (size_t)c->max_seq * row;
   for (int i = 0; i < n; i++) {     /* sequential, like the reference loop (reference: spec_tree.py:126-128) */

@@ -38,7 +38,16 @@ struct fb_ctx {
   void* vrope;                                                      // verify: (cos, sin) per (token, rotation pair)
   int max_fly;                                                      // max_fly 0: chosen by the bytes of a layer (fly_for)
   CUtensorMap kmap, vmap;                                           // the caches as tensors (make_kv_maps)
+  bool kv4_bound;                                                   // the 4-bit cache is the one that is used: its first layer and one sequence, ...
+  fb_kv4_seqs kv4;
+  int64_t kv4_layer;                                                // ... bytes of a layer, ...
+  const uint64_t* kv4_freq;
+  uint16_t* kv4_new;                                                // ... a layer's new keys and values ahead of their rounding, bf16 [2][kPromptRows][n_kv * HD],
+  float* kv4_logits;                                                // and what a decode step on it needs: logits, token
+  int32_t* kv4_token;
 };
+
+inline bool has_kv(const fb_ctx* c) { return c->kv4_bound || c->kc; }
 
 inline int cuda_fail(fb_ctx* c, cudaError_t e) {
   if (c) c->last_cuda_error = (int)e;
@@ -82,6 +91,13 @@ void pass_free(fb_ctx* c);
 // one stacked weight matrix in the layouts the passes read (order / arg / orows as in fb_repack)
 cudaError_t pass_bind_matrix(fb_ctx* c, int which, const void* q, const void* s, const void* z, int layers, int rows, int k, int order,
                              int arg, int orows, cudaStream_t st);
+
+// one decode step on the 4-bit cache: the M-token pass with one token, and the arg-max
+int pass_decode(fb_ctx* c, int32_t token, const int32_t* d_token, void* d_h, int32_t pos, float* d_logits, int32_t* d_next, cudaStream_t st);
+
+// ---- the 4-bit cache (fb_kv4.cu), with the context's limit of waits
+int kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n_head, int32_t max_new, int32_t max_len, const uint8_t* d_amask, int32_t mask_ld,
+               float scale, void* d_out, int64_t o_ld, unsigned spin_limit, cudaStream_t st);
 
 // ---- the decode kernels of tensor-parallel ranks (fb_decode_tp.cu), by index into fb_api.cu's table
 const void* decode_tp_kernel(int id);

@@ -155,6 +155,13 @@ int fb_kv4_move(const fb_kv4_seqs* s, int32_t n_layer, int64_t layer_bytes, cons
 
 int fb_kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n_head, int32_t max_new, int32_t max_len, const uint8_t* d_amask,
                   int32_t mask_ld, float scale, void* d_out, int64_t o_ld, void* stream) {
+  return kv4_attend(s, d_q, q_ld, n_head, max_new, max_len, d_amask, mask_ld, scale, d_out, o_ld, 4000000u, (cudaStream_t)stream);
+}
+
+}  // extern "C"
+
+int kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n_head, int32_t max_new, int32_t max_len, const uint8_t* d_amask, int32_t mask_ld,
+               float scale, void* d_out, int64_t o_ld, unsigned spin_limit, cudaStream_t st) {
   Kv4Attend p;
   const int rc = take_seqs(s, 1, p.S);
   if (rc != FB_OK) return rc;
@@ -168,8 +175,7 @@ int fb_kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n
   if (!g.ok || !sms) return FB_ERR_CUDA;
   p.q = (const uint16_t*)d_q; p.out = (uint16_t*)d_out; p.q_ld = q_ld; p.o_ld = o_ld; p.amask = d_amask; p.mask_ld = mask_ld;
   p.nh = n_head; p.R = n_head / s->n_kv_head; p.max_new = max_new < s->n_tokens ? max_new : s->n_tokens;
-  p.scale = scale * 1.4426950408889634f; p.spin_limit = 4000000u;
-  cudaStream_t st = (cudaStream_t)stream;
+  p.scale = scale * 1.4426950408889634f; p.spin_limit = spin_limit;
   const bool one = (int64_t)p.max_new * p.R <= 8;
   switch (s->head_dim) {
     case 64: return done(one ? launch_few<64, 1, 16>(p, max_len, sms, st) : launch_few<64, 2, 8>(p, max_len, sms, st));
@@ -177,5 +183,3 @@ int fb_kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n
     default: return done(one ? launch_few<128, 1, 16>(p, max_len, sms, st) : launch_few<128, 2, 8>(p, max_len, sms, st));
   }
 }
-
-}  // extern "C"

@@ -122,16 +122,18 @@ int run_tc_pass(fb_ctx* c, const int32_t* d_tokens, const void* d_h, const int32
   const fb_model_desc& d = c->d;
   const int D = d.dim, FF = d.ffn, HD = d.head_dim, QD = d.n_head * HD, QKV = (d.n_head + 2 * d.n_kv_head) * HD, sms = c->sm_count;
   const bool hz = d.has_zeros != 0;
-  const bool tree = token_tile(M) <= 64;
+  const bool kv4 = c->kv4_bound, tree = token_tile(M) <= 64 && !kv4;
+  fb_kv4_seqs seqs = c->kv4;
+  seqs.cached = pos; seqs.n_tokens = M;
   const size_t tQ = tc_matrix_bytes(QKV, D, hz), tO = tc_matrix_bytes(D, QD, hz), tG = tc_matrix_bytes(2 * FF, D, hz),
                tF = tc_matrix_bytes(D, FF, hz);
   FB_CUDA(c, launch_pdl(v_embed, dim3(M), dim3(256), 0, st, d_tokens, (const uint16_t*)c->embed, (const uint16_t*)d_h, c->vh,
                         D, d.vocab, d.emb_mult, &c->status->code));
-  FB_CUDA(c, launch_pdl(v_rope_table, dim3(M), dim3(64), 0, st, d_depth, (const float*)c->invf, pos, HD / 2, (float2*)c->vrope));
+  FB_CUDA(c, launch_pdl(v_rope_table, dim3(M), dim3(64), 0, st, d_depth, (const float*)(kv4 ? nullptr : c->invf), pos, HD / 2, (float2*)c->vrope));
   VtcParams t;
   memset(&t, 0, sizeof(t));
   t.M = M; t.status = c->status; t.spin_limit = c->spin_limit;
-  t.rope = (const float2*)c->vrope; t.n_head = d.n_head; t.nkv = d.n_kv_head; t.pos = pos; t.head_dim = HD;
+  t.rope = (const float2*)c->vrope; t.n_head = d.n_head; t.nkv = d.n_kv_head; t.pos = kv4 ? 0 : pos; t.head_dim = HD;
   t.resid = d.resid_mult; t.logits_scaling = d.logits_scaling; t.h = c->vh; t.q = c->vq; t.act = c->vact; t.fa = c->vfa;
   t.logits = d_logits;
   auto norm = [&](const void* w, uint16_t* feat, const unsigned* norms) {
@@ -142,14 +144,23 @@ int run_tc_pass(fb_ctx* c, const int32_t* d_tokens, const void* d_h, const int32
   };
   if (D > 8 * 256 * 2) return FB_ERR_SHAPE;
   for (int l = 0; l < d.n_layer; l++) {
-    uint16_t* kcl = (uint16_t*)c->kc + (size_t)l * c->max_seq * d.n_kv_head * HD;
-    uint16_t* vcl = (uint16_t*)c->vc + (size_t)l * c->max_seq * d.n_kv_head * HD;
+    const size_t kw = (size_t)d.n_kv_head * HD;
+    uint16_t* kcl = kv4 ? c->kv4_new : (uint16_t*)c->kc + (size_t)l * c->max_seq * kw;
+    uint16_t* vcl = kv4 ? c->kv4_new + kPromptRows * kw : (uint16_t*)c->vc + (size_t)l * c->max_seq * kw;
     FB_CUDA(c, norm((const uint16_t*)c->n1 + (size_t)l * D, nullptr, nullptr));
     t.w = c->t_qkv + l * tQ; t.rows = QKV; t.K = D; t.kc = kcl; t.vc = vcl; t.fx = c->vfx;
     FB_CUDA(c, launch_vtc<EPI_QKV>(t, c->m_xn, hz, sms, st));
     // trees: the O GEMM converts the attention output to fp16 on its way in; prompts, whose activations come by tensor copies, have it
-    // converted in place
-    FB_CUDA(c, launch_vattn_tc(c, kcl, vcl, d_amask, pos, M, tree, st));
+    // converted in place (and so do all passes on a 4-bit cache)
+    if (kv4) {
+      int rc = fb_kv4_append(&seqs, c->vq, QD, kcl, kw, vcl, kw, d.n_head, d_depth, c->kv4_freq, c->vq, QD, st);
+      if (rc == FB_OK)
+        rc = kv4_attend(&seqs, c->vq, QD, d.n_head, M, pos + M, d_amask, M, d.attn_scale, c->vao, QD, c->spin_limit, st);
+      if (rc != FB_OK) return rc == FB_ERR_CUDA ? cuda_fail(c, cudaGetLastError()) : rc;
+      seqs.d_pool = (uint8_t*)seqs.d_pool + c->kv4_layer;
+    } else {
+      FB_CUDA(c, launch_vattn_tc(c, kcl, vcl, d_amask, pos, M, tree, st));
+    }
     if (!tree) FB_CUDA(c, launch_pdl(v_row_f16, dim3(M), dim3(256), 0, st, c->vao, c->vfao, QD));
     t.w = c->t_o + l * tO; t.rows = D; t.K = QD; t.out_ld = D; t.fx = c->vfao;
     t.xbf = tree ? c->vao : nullptr; t.amax = tree ? c->vamax : nullptr;
@@ -171,7 +182,24 @@ int run_tc_pass(fb_ctx* c, const int32_t* d_tokens, const void* d_h, const int32
   return FB_OK;
 }
 
+__global__ void set_token(int32_t* to, int32_t token) {
+  pdl_begin(true);
+  *to = token;
+}
+
 }  // namespace
+
+int pass_decode(fb_ctx* c, int32_t token, const int32_t* d_token, void* d_h, int32_t pos, float* d_logits, int32_t* d_next, cudaStream_t st) {
+  if (!d_token && !d_h) {
+    FB_CUDA(c, launch_pdl(set_token, dim3(1), dim3(1), 0, st, c->kv4_token, token));
+    d_token = c->kv4_token;
+  }
+  float* logits = d_logits || !d_next ? d_logits : c->kv4_logits;
+  const int rc = run_tc_pass(c, d_h ? nullptr : d_token, d_h, nullptr, nullptr, 1, pos, logits, nullptr, st);
+  if (rc != FB_OK) return rc;
+  if (d_h) FB_CUDA(c, cudaMemcpyAsync(d_h, c->vh, (size_t)c->d.dim * 2, cudaMemcpyDeviceToDevice, st));
+  return d_next ? fb_sample(logits, c->d.vocab, 1, 0, 0.f, 0, 0, 0, d_next, st) : FB_OK;
+}
 
 cudaError_t pass_alloc(fb_ctx* c) {
   const fb_model_desc& d = c->d;
@@ -197,7 +225,7 @@ cudaError_t pass_alloc(fb_ctx* c) {
 
 void pass_free(fb_ctx* c) {
   void* ptrs[] = {c->vh, c->vxn, c->vq, c->vao, c->vact, c->t_qkv, c->t_o, c->t_gu, c->t_d, c->t_lm, c->vrope,
-                  c->vfx, c->vfao, c->vfa, c->vfa_inv, c->vamax, c->gu_norms};
+                  c->vfx, c->vfao, c->vfa, c->vfa_inv, c->vamax, c->gu_norms, c->kv4_new, c->kv4_logits, c->kv4_token};
   for (void* p : ptrs)
     if (p) cudaFree(p);
 }
@@ -220,7 +248,7 @@ extern "C" {
 
 int fb_prefill(fb_ctx* c, const int32_t* d_tokens, int32_t n, int32_t pos, float* d_logits, void* d_feat, void* stream) {
   if (!c || !d_tokens || n < 1 || ((uintptr_t)d_feat & 15)) return FB_ERR_ARG;       /* features are stored 16 bytes at a time */
-  if (!c->weights_bound || !c->kc) return FB_ERR_STATE;
+  if (!c->weights_bound || !has_kv(c)) return FB_ERR_STATE;
   if (c->tp_size > 1 || !c->embed) return FB_ERR_STATE;
   if (pos < 0 || n > c->max_seq - pos) return FB_ERR_RANGE;
   DeviceGuard g(c->device);
@@ -239,7 +267,7 @@ int fb_prefill(fb_ctx* c, const int32_t* d_tokens, int32_t n, int32_t pos, float
 int fb_verify(fb_ctx* c, const int32_t* d_tokens, const void* d_h, const int32_t* d_depth, const uint8_t* d_amask,
               int32_t M, int32_t pos, float* d_logits, void* d_feat, void* stream) {
   if (!c || !d_depth || !d_amask || (!d_tokens && !d_h) || ((uintptr_t)d_feat & 15)) return FB_ERR_ARG;
-  if (!c->weights_bound || !c->kc) return FB_ERR_STATE;
+  if (!c->weights_bound || !has_kv(c)) return FB_ERR_STATE;
   if (c->tp_size > 1) return FB_ERR_STATE;           /* a tensor-parallel rank holds slices only */
   if (!d_h && !c->embed) return FB_ERR_STATE;
   if (M < 1 || M > 64) return FB_ERR_RANGE;          /* never fall through to another M (reference: result.md:112-113) */

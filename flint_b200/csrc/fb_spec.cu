@@ -112,8 +112,13 @@ int fb_accept_tree(const int32_t* d_cand, const int32_t* d_parent, const int32_t
 }
 
 int fb_kv_compact(fb_ctx* c, const int32_t* d_accept, int32_t pos, void* stream) {
-  if (!c || !c->kc || !d_accept) return FB_ERR_ARG;
+  if (!c || !has_kv(c) || !d_accept) return FB_ERR_ARG;
   if (pos < 0 || pos >= c->max_seq) return FB_ERR_RANGE;
+  if (c->kv4_bound) {
+    fb_kv4_seqs s = c->kv4;
+    s.cached = pos;
+    return fb_kv4_compact(&s, c->d.n_layer, c->kv4_layer, d_accept, 64, stream);
+  }
   const fb_model_desc& d = c->d;
   DeviceGuard g(c->device);
   const int row = d.n_kv_head * d.head_dim;

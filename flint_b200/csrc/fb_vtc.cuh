@@ -235,14 +235,14 @@ __global__ void __launch_bounds__(256) v_row_f16(uint16_t* x, float* fx, int D) 
 }
 
 // cos / sin of every (token, rotation pair): the QKV epilogue reads them instead of evaluating sincosf per output.
-// depth == nullptr: a chain, token m sits at position pos + m
+// depth == nullptr: a chain, token m sits at position pos + m. invf == nullptr: no rotation (a 4-bit cache's append rotates)
 __global__ void v_rope_table(const int32_t* depth, const float* invf, int pos, int half, float2* out) {
   const int m = blockIdx.x;
   pdl_trigger();
   pdl_wait();
   for (int i = threadIdx.x; i < half; i += blockDim.x) {
-    float sn, cs;
-    sincosf((float)(pos + (depth ? depth[m] : m)) * invf[i], &sn, &cs);
+    float sn = 0.f, cs = 1.f;
+    if (invf) sincosf((float)(pos + (depth ? depth[m] : m)) * invf[i], &sn, &cs);
     out[(size_t)m * half + i] = make_float2(cs, sn);
   }
 }

@@ -45,8 +45,16 @@ class DecodeEngine:
 
     def __init__(self, cfg: ModelArgs, packed: Dict[str, torch.Tensor], max_seq: Optional[int] = None,
                  device: Optional[torch.device] = None, kc: Optional[torch.Tensor] = None,
-                 vc: Optional[torch.Tensor] = None, tp_rank: int = 0, tp_size: int = 1):
-        """`packed` holds this rank's slice when tp_size > 1 (flint_b200.tp.shard_packed); cfg is the full model."""
+                 vc: Optional[torch.Tensor] = None, tp_rank: int = 0, tp_size: int = 1, kv_bits: int = 16, cache=None):
+        """`packed` holds this rank's slice when tp_size > 1 (flint_b200.tp.shard_packed); cfg is the full model. kv_bits 4: the K/V cache is a paged one of 4 bits
+        a number (`cache`, a flint_b200.kv4.KvCache4 of the model's layers and one sequence, or one of its own with room for max_seq): a quarter of the
+        memory and of the bytes that a token's attention reads; every pass then runs as the M-token pass, decode steps too."""
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits is 16 or 4, not {kv_bits}")
+        if kv_bits == 4 and (tp_size > 1 or kc is not None or vc is not None):
+            raise ValueError("a 4-bit cache is a KvCache4, on one GPU")
+        if kv_bits == 16 and cache is not None:
+            raise ValueError("`cache` is the 4-bit cache: kv_bits=4")
         self.lib = _lib.load()
         if not torch.cuda.is_available():
             raise RuntimeError("flint_b200 needs a CUDA device (sm_100a); there is no CPU path")
@@ -84,12 +92,16 @@ class DecodeEngine:
                 setattr(w, name, t.data_ptr())
         _lib.check(self.lib.fb_bind_weights(self._ctx, ctypes.byref(w), _raw_stream(self.dev_index)), "fb_bind_weights")
         torch.cuda.synchronize(self.device)
+        self._logits = torch.empty(cfg.vocab_size, dtype=torch.float32, device=self.device)
+        self._next = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.kc = self.vc = self.cache = None
+        if kv_bits == 4:
+            self.bind_kv4(cache if cache is not None else self._own_cache())
+            return
         shape = (cfg.n_layer, self.max_seq, self.n_kv_local, cfg.head_dim)
         self.kc = kc if kc is not None else torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
         self.vc = vc if vc is not None else torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
         self.bind_kv(self.kc, self.vc)
-        self._logits = torch.empty(cfg.vocab_size, dtype=torch.float32, device=self.device)
-        self._next = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     # ------------------------------------------------------------------ plumbing
     def bind_kv(self, kc: torch.Tensor, vc: torch.Tensor):
@@ -99,6 +111,24 @@ class DecodeEngine:
                 raise ValueError(f"KV cache must be contiguous bf16 {want} on {self.device}")
         self.kc, self.vc, self.max_seq = kc, vc, kc.shape[1]
         _lib.check(self.lib.fb_bind_kv(self._ctx, _ptr(kc), _ptr(vc), self.max_seq), "fb_bind_kv")
+        self.cache = None
+
+    def _own_cache(self):
+        from .kv4 import PAGE, KvCache4
+        pages = (self.max_seq + PAGE - 1) // PAGE
+        table = torch.arange(pages, dtype=torch.int32, device=self.device).view(1, pages)
+        return KvCache4(self.cfg.n_layer, pages, self.cfg.n_local_heads, self.cfg.head_dim, table, rope_base=self.cfg.rope_base)
+
+    def bind_kv4(self, cache):
+        """The passes use this 4-bit cache (one sequence, the model's layers, heads and rotation) from here on, instead of the one bound before."""
+        cfg = self.cfg
+        if (cache.n_layer, cache.n_kv, cache.head_dim, cache.table.shape[0]) != (cfg.n_layer, self.n_kv_local, cfg.head_dim, 1) or cache.device != self.device:
+            raise ValueError(f"the 4-bit cache must have {cfg.n_layer} layers, {self.n_kv_local} kv heads of {cfg.head_dim} and one sequence, on {self.device}")
+        if cache.freq is None:
+            raise ValueError("the 4-bit cache needs the model's rotation (rope_base)")
+        s = cache._one(0, 0)
+        _lib.check(self.lib.fb_bind_kv4(self._ctx, ctypes.byref(s), cache.layer_bytes, _ptr(cache.freq)), "fb_bind_kv4")
+        self.cache, self.kc, self.vc, self.max_seq = cache, None, None, cache.slots
 
     # ------------------------------------------------------------------ tensor parallel wiring
     def tp_export(self) -> bytes:

@@ -17,16 +17,20 @@ from .engine import DecodeEngine
 
 
 class Transformer:
-    def __init__(self, config: ModelArgs) -> None:
+    def __init__(self, config: ModelArgs, kv_bits: int = 16) -> None:
+        """kv_bits 4: a paged K/V cache of 4 bits a number (DecodeEngine)."""
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits is 16 or 4, not {kv_bits}")
         self.config = config
+        self.kv_bits = kv_bits
         self.packed: Optional[Dict[str, torch.Tensor]] = None
         self.engine: Optional[DecodeEngine] = None
         self.max_batch_size = -1
         self.max_seq_length = -1
 
     @classmethod
-    def from_name(cls, name: str) -> "Transformer":
-        return cls(ModelArgs.from_name(name))
+    def from_name(cls, name: str, kv_bits: int = 16) -> "Transformer":
+        return cls(ModelArgs.from_name(name), kv_bits)
 
     # ---- weights: a packed dict as the reference's load_packed returns (reference: chat.py:32-52) ----
     def load_packed(self, packed: Dict[str, torch.Tensor]) -> "Transformer":
@@ -45,7 +49,7 @@ class Transformer:
         if self.engine is not None and self.max_seq_length >= max_seq_length:
             return
         max_seq_length = (max_seq_length + 7) // 8 * 8          # reference: engine/model.py:118
-        self.engine = DecodeEngine(self.config, self.packed, max_seq=max_seq_length)
+        self.engine = DecodeEngine(self.config, self.packed, max_seq=max_seq_length, kv_bits=self.kv_bits)
         self.max_batch_size, self.max_seq_length = 1, max_seq_length
 
     def forward(self, idx: torch.Tensor, input_pos: torch.Tensor, return_hidden: bool = False):

@@ -27,11 +27,12 @@ def main():
     ap.add_argument("--D", type=int, default=6)
     ap.add_argument("--W", type=int, default=32)
     ap.add_argument("--max-new", type=int, default=64)
+    ap.add_argument("--kv-bits", type=int, default=16, choices=(4, 16), help="bits of a number of the K/V cache")
     ap.add_argument("--selftest", action="store_true")
     ap.add_argument("--check", action="store_true", help="compare with plain greedy decoding of the same prompt")
     a = ap.parse_args()
     torch.set_grad_enabled(False)
-    model = Transformer.from_name(a.config).load_synthetic(seed=0)
+    model = Transformer.from_name(a.config, a.kv_bits).load_synthetic(seed=0)
     cfg = model.config
     if a.draft:
         ck = torch.load(a.draft, map_location="cpu")
