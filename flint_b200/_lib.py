@@ -116,7 +116,9 @@ _PROTOS = {
                                      ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
                                      ctypes.c_void_p]),
     "fb_kv4_attend": (ctypes.c_int, [ctypes.POINTER(Kv4Seqs), ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
-                                     ctypes.c_void_p, ctypes.c_int32, ctypes.c_float, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+                                     ctypes.c_void_p, ctypes.c_int32, ctypes.c_float, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t,
+                                     ctypes.c_void_p]),
+    "fb_kv4_attend_bytes": (ctypes.c_size_t, [ctypes.POINTER(Kv4Seqs), ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
     "fb_kv4_read": (ctypes.c_int, [ctypes.POINTER(Kv4Seqs), ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "fb_kv4_compact": (ctypes.c_int, [ctypes.POINTER(Kv4Seqs), ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p]),
     "fb_kv4_move": (ctypes.c_int, [ctypes.POINTER(Kv4Seqs), ctypes.c_int32, ctypes.c_int64, ctypes.POINTER(ctypes.c_int32),

@@ -469,6 +469,10 @@ int fb_bind_kv4(fb_ctx* c, const fb_kv4_seqs* s, int64_t layer_bytes, const uint
   if (!c->kv4_new) FB_CUDA(c, dmalloc(&c->kv4_new, (size_t)2 * kPromptRows * d.n_kv_head * d.head_dim * 2));
   if (!c->kv4_logits) FB_CUDA(c, dmalloc(&c->kv4_logits, (size_t)d.vocab * 4));
   if (!c->kv4_token) FB_CUDA(c, dmalloc(&c->kv4_token, 4));
+  if (!c->kv4_work) {
+    c->kv4_work_bytes = kv4_attend_most(d.n_kv_head, d.head_dim, c->sm_count);
+    FB_CUDA(c, dmalloc(&c->kv4_work, c->kv4_work_bytes));
+  }
   c->kv4 = *s;
   c->kv4.d_start = c->kv4.d_cached = nullptr;
   c->kv4.d_status = (int32_t*)c->status;

@@ -1,6 +1,8 @@
 // extern "C" entry points of the 4-bit paged K/V cache: append, attention, read-back, moves.
 // No torch types, no CPU fallback: a failed CUDA call or an unsupported shape is an error code.
 #include <string.h>
+#include <stdlib.h>
+#include <stdio.h>
 
 #include "../../include/flint_b200.h"
 #include "fb_ctx.hpp"
@@ -10,12 +12,25 @@ using namespace fb;
 
 namespace {
 
+constexpr int kFewWarps = 7;                       // that compute, of a CTA of kv4_attn_few; an SM holds two CTAs
+
 int device_sms(int dev) {
   static int sms[64] = {};
   if (dev < 0 || dev >= 64) return 0;
   if (!sms[dev] && cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
   return sms[dev];
 }
+
+// The call's device, made current only where it is not (that alone takes half a microsecond)
+struct OnDevice {
+  int prev = 0;
+  bool ok = false, moved = false;
+  explicit OnDevice(int dev) {
+    if (cudaGetDevice(&prev) != cudaSuccess) return;
+    ok = prev == dev || (moved = cudaSetDevice(dev) == cudaSuccess);
+  }
+  ~OnDevice() { if (moved) cudaSetDevice(prev); }
+};
 
 // FB_OK and the kernels' view of the sequences, or why not
 int take_seqs(const fb_kv4_seqs* s, int rows_of_tokens, Kv4Seqs& S) {
@@ -32,29 +47,57 @@ int take_seqs(const fb_kv4_seqs* s, int rows_of_tokens, Kv4Seqs& S) {
 }
 int done(cudaError_t e) { return e == cudaSuccess ? FB_OK : FB_ERR_CUDA; }
 
+// How an attention of few rows is cut. rows: query rows of a group; groups: of all sequences, at most; ctas: of a grid without clusters, at most.
+// A group's positions are shared by a cluster (one launch) while a warp of a cluster of eight has no more than six units; by as many CTAs as the GPU holds and a
+// second launch that joins them, beyond that. (With one CTA of 16-row groups per SM the GPU holds 15 clusters of 8, but 36 of 4.) Microseconds, one sequence, eight kv heads, cluster / second launch: 1000 positions 5.5 / 8.2, 4000 6.7 / 8.5,
+// 32768 20.5 / 13.1 (heads of 80). Of a batch no positions are shared until a warp would have more than 12 units: 48 sequences of up to 2000
+// positions 17.8 / 22.7, 24 of up to 8000 51 / 18.3 (over 148 parts; over 296 22.1).
+struct Kv4Geometry { int rows; int64_t groups, ctas; int nsplit, slots, chunk; };
+Kv4Geometry few_geometry(int n_seq, int n_tokens, int nkv, int r, int max_new, int max_len, int sms) {
+  Kv4Geometry g{(int64_t)max_new * r <= 8 ? 8 : 16, 0, 0, 1, 0, 8};
+  g.groups = n_seq == 1 ? ((int64_t)n_tokens * r + g.rows - 1) / g.rows : (int64_t)n_tokens * r / g.rows + n_seq;
+  const int64_t units = ((int64_t)max_len + 31) / 32, items = g.groups * nkv;
+  if (n_seq == 1) {
+    while (g.nsplit < 8 && items * g.nsplit * 2 <= (g.nsplit == 4 ? sms * 2 / 3 : sms) && units >= g.nsplit * 2 * 4) g.nsplit *= 2;
+    if (units > (int64_t)6 * kFewWarps * g.nsplit && items * g.nsplit <= sms) { g.nsplit = 1; g.slots = 2 * sms; }
+  } else if (units > 12 * kFewWarps && items <= 8 * (int64_t)sms) {
+    g.slots = sms;
+  }
+  g.ctas = items + g.slots;
+  return g;
+}
+size_t few_work(const Kv4Geometry& g, int hd) { return g.slots ? (size_t)g.ctas * g.rows * (hd + 4) * 4 : 0; }
+
 // rows of 16-bit numbers that are read 16 bytes at a time
 bool rows_ok(const void* p, int64_t ld, int64_t width) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld >= width; }
 
-template <int HD, int NQ, int W>
-cudaError_t launch_few(Kv4Attend p, int max_len, int sms, cudaStream_t st) {
-  using F = Kv4Few<HD, NQ, W>;
-  static bool configured[64] = {};
+template <class K>
+cudaError_t configure_few(K k, int smem, bool (&configured)[64]) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  auto k = kv4_attn_few<HD, NQ, W>;
-  if (!configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, F::TOTAL);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-    configured[dev] = true;
+  if (configured[dev]) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  configured[dev] = e == cudaSuccess;
+  return e;
+}
+template <int HD, int NQ, int W>
+cudaError_t launch_few(Kv4Attend p, const Kv4Geometry& g, cudaStream_t st) {
+  using F = Kv4Few<HD, NQ, W>;
+  static bool done_c[64] = {}, done_s[64] = {};
+  p.nsplit = g.nsplit; p.slots = g.slots; p.chunk = g.chunk;
+  if (g.groups * g.nsplit > 0x7fffffff || g.ctas > 0x7fffffff) return cudaErrorInvalidValue;
+  const dim3 block(W * 32 + 32);
+  if (g.nsplit > 1) {
+    const cudaError_t e = configure_few(kv4_attn_few<HD, NQ, W, true>, F::TOTAL, done_c);
+    return e != cudaSuccess ? e : launch_pdl_cluster(kv4_attn_few<HD, NQ, W, true>, dim3((unsigned)(g.groups * g.nsplit), (unsigned)p.S.nkv), block,
+                                                     (size_t)F::TOTAL, st, (unsigned)g.nsplit, p);
   }
-  p.groups = (int)(((int64_t)p.max_new * p.R + F::ROWS - 1) / F::ROWS);
-  const int64_t items = (int64_t)p.S.n_seq * p.groups, units = ((int64_t)max_len + F::U - 1) / F::U;
-  int ns = 1;
-  while (ns < 16 && items * p.S.nkv * ns * 2 <= sms && units >= (int64_t)ns * 2 * W) ns *= 2;
-  p.nsplit = ns;
-  if (items * ns > 0x7fffffff) return cudaErrorInvalidValue;
-  return launch_pdl_cluster(k, dim3((unsigned)(items * ns), (unsigned)p.S.nkv), dim3(W * 32), (size_t)F::TOTAL, st, (unsigned)ns, p);
+  cudaError_t e = configure_few(kv4_attn_few<HD, NQ, W, false>, F::TOTAL, done_s);
+  if (e == cudaSuccess) e = launch_pdl(kv4_attn_few<HD, NQ, W, false>, dim3((unsigned)g.ctas), block, (size_t)F::TOTAL, st, p);
+  if (e != cudaSuccess || !g.slots) return e;
+  if (p.S.n_seq == 1)
+    return launch_pdl(kv4_join<HD, F::ROWS, F::U, 8>, dim3((unsigned)g.groups, (unsigned)p.S.nkv, F::ROWS), dim3(256), 0, st, p);
+  return launch_pdl(kv4_join<HD, F::ROWS, F::U, 1>, dim3((unsigned)g.groups, (unsigned)p.S.nkv), dim3(F::ROWS * 32), 0, st, p);
 }
 
 }  // namespace
@@ -75,7 +118,7 @@ int fb_kv4_append(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, const voi
   const int64_t hd = s->head_dim, kw = hd * s->n_kv_head, qw = hd * n_head;
   if (!d_k || !d_v || !rows_ok(d_k, k_ld, kw) || !rows_ok(d_v, v_ld, kw) || ((uintptr_t)d_freq & 7) || ((uintptr_t)d_depth & 3)) return FB_ERR_ARG;
   if (d_q && (!d_q_out || n_head < 1 || !rows_ok(d_q, q_ld, qw) || !rows_ok(d_q_out, qo_ld, qw))) return FB_ERR_ARG;
-  DeviceGuard g(s->device);
+  OnDevice g(s->device);
   const int sms = device_sms(s->device);
   if (!g.ok || !sms) return FB_ERR_CUDA;
   p.q = (const uint16_t*)d_q; p.k = (const uint16_t*)d_k; p.v = (const uint16_t*)d_v; p.q_out = (uint16_t*)d_q_out;
@@ -97,7 +140,7 @@ int fb_kv4_read(const fb_kv4_seqs* s, int32_t n_layer, int64_t layer_bytes, floa
   if (rc != FB_OK) return rc;
   if (n_layer < 1 || n_layer > 65535 || layer_bytes < 0 || layer_bytes % 16 || ((uintptr_t)d_k & 15) || ((uintptr_t)d_v & 15)) return FB_ERR_ARG;
   if (s->n_tokens == 0 || s->n_seq == 0 || (!d_k && !d_v)) return FB_OK;
-  DeviceGuard g(s->device);
+  OnDevice g(s->device);
   if (!g.ok) return FB_ERR_CUDA;
   p.k = d_k; p.v = d_v; p.layer = (size_t)layer_bytes;
   const dim3 grid(s->n_tokens, n_layer), block(256);
@@ -125,7 +168,7 @@ int fb_kv4_compact(const fb_kv4_seqs* s, int32_t n_layer, int64_t layer_bytes, c
   if (rc != FB_OK) return rc;
   if (!d_accept || ((uintptr_t)d_accept & 3) || most < 0 || n_layer < 1 || n_layer > 65535 || layer_bytes < 0 || layer_bytes % 16 || s->d_cached) return FB_ERR_ARG;
   if (s->cached > s->table_ld * kPage - 1) return FB_ERR_RANGE;
-  DeviceGuard g(s->device);
+  OnDevice g(s->device);
   if (!g.ok) return FB_ERR_CUDA;
   p.layer = (size_t)layer_bytes; p.accept = d_accept; p.pos = s->cached; p.most = most;
   return launch_move(s, p, n_layer, (cudaStream_t)stream);
@@ -140,7 +183,7 @@ int fb_kv4_move(const fb_kv4_seqs* s, int32_t n_layer, int64_t layer_bytes, cons
   const int64_t slots = (int64_t)s->table_ld * kPage;
   for (int i = 0; i < n; i++)
     if (src[i] < 0 || dst[i] < 0 || src[i] >= slots || dst[i] >= slots) return FB_ERR_RANGE;
-  DeviceGuard g(s->device);
+  OnDevice g(s->device);
   if (!g.ok) return FB_ERR_CUDA;
   p.layer = (size_t)layer_bytes;
   for (int i0 = 0; i0 < n; i0 += 64) {                           // the moves of a launch travel in its parameters
@@ -154,14 +197,14 @@ int fb_kv4_move(const fb_kv4_seqs* s, int32_t n_layer, int64_t layer_bytes, cons
 }
 
 int fb_kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n_head, int32_t max_new, int32_t max_len, const uint8_t* d_amask,
-                  int32_t mask_ld, float scale, void* d_out, int64_t o_ld, void* stream) {
-  return kv4_attend(s, d_q, q_ld, n_head, max_new, max_len, d_amask, mask_ld, scale, d_out, o_ld, 4000000u, (cudaStream_t)stream);
+                  int32_t mask_ld, float scale, void* d_out, int64_t o_ld, void* d_work, size_t work_bytes, void* stream) {
+  return kv4_attend(s, d_q, q_ld, n_head, max_new, max_len, d_amask, mask_ld, scale, d_out, o_ld, (float*)d_work, work_bytes, 4000000u, (cudaStream_t)stream);
 }
 
 }  // extern "C"
 
 int kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n_head, int32_t max_new, int32_t max_len, const uint8_t* d_amask, int32_t mask_ld,
-               float scale, void* d_out, int64_t o_ld, unsigned spin_limit, cudaStream_t st) {
+               float scale, void* d_out, int64_t o_ld, float* work, size_t work_bytes, unsigned spin_limit, cudaStream_t st) {
   Kv4Attend p;
   const int rc = take_seqs(s, 1, p.S);
   if (rc != FB_OK) return rc;
@@ -170,16 +213,29 @@ int kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n_he
   if (n_head < 1 || n_head % s->n_kv_head) return FB_ERR_SHAPE;
   if (!d_q || !d_out || !rows_ok(d_q, q_ld, qw) || !rows_ok(d_out, o_ld, qw) || max_new < 1 || max_len < 1 || (d_amask && mask_ld < 1)) return FB_ERR_ARG;
   if ((int64_t)s->n_tokens * (n_head / s->n_kv_head) > 0x7fffffff - 256) return FB_ERR_RANGE;      /* rows of a sequence */
-  DeviceGuard g(s->device);
+  OnDevice g(s->device);
   const int sms = device_sms(s->device);
   if (!g.ok || !sms) return FB_ERR_CUDA;
   p.q = (const uint16_t*)d_q; p.out = (uint16_t*)d_out; p.q_ld = q_ld; p.o_ld = o_ld; p.amask = d_amask; p.mask_ld = mask_ld;
-  p.nh = n_head; p.R = n_head / s->n_kv_head; p.max_new = max_new < s->n_tokens ? max_new : s->n_tokens;
+  p.nh = n_head; p.R = n_head / s->n_kv_head;
   p.scale = scale * 1.4426950408889634f; p.spin_limit = spin_limit;
-  const bool one = (int64_t)p.max_new * p.R <= 8;
+  const Kv4Geometry geo = few_geometry(s->n_seq, s->n_tokens, s->n_kv_head, p.R, max_new < s->n_tokens ? max_new : s->n_tokens, max_len, sms);
+  if (few_work(geo, s->head_dim) > work_bytes || ((uintptr_t)work & 15)) return FB_ERR_ARG;
+  p.work = work;
+  const bool one = geo.rows == 8;
   switch (s->head_dim) {
-    case 64: return done(one ? launch_few<64, 1, 16>(p, max_len, sms, st) : launch_few<64, 2, 8>(p, max_len, sms, st));
-    case 80: return done(one ? launch_few<80, 1, 16>(p, max_len, sms, st) : launch_few<80, 2, 8>(p, max_len, sms, st));
-    default: return done(one ? launch_few<128, 1, 16>(p, max_len, sms, st) : launch_few<128, 2, 8>(p, max_len, sms, st));
+    case 64: return done(one ? launch_few<64, 1, kFewWarps>(p, geo, st) : launch_few<64, 2, 7>(p, geo, st));
+    case 80: return done(one ? launch_few<80, 1, kFewWarps>(p, geo, st) : launch_few<80, 2, 7>(p, geo, st));
+    default: return done(one ? launch_few<128, 1, kFewWarps>(p, geo, st) : launch_few<128, 2, 7>(p, geo, st));
   }
+}
+
+// one sequence is split over clusterless CTAs only while its row groups are fewer than the SMs
+size_t kv4_attend_most(int n_kv_head, int head_dim, int sms) { return (size_t)(3 * sms + n_kv_head) * 16 * (head_dim + 4) * 4; }
+
+size_t fb_kv4_attend_bytes(const fb_kv4_seqs* s, int32_t n_head, int32_t max_new, int32_t max_len) {
+  if (!s || s->n_kv_head < 1 || s->n_kv_head > 65535 || n_head < 1 || n_head % s->n_kv_head || max_new < 1 || max_len < 1 || s->n_seq < 0) return 0;
+  const int sms = device_sms(s->device);
+  if (!sms) return 0;
+  return few_work(few_geometry(s->n_seq, s->n_tokens, s->n_kv_head, n_head / s->n_kv_head, max_new < s->n_tokens ? max_new : s->n_tokens, max_len, sms), s->head_dim);
 }

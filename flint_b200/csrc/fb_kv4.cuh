@@ -12,6 +12,8 @@
 //      The words of a pair of positions in a row, tails behind, 16-byte (HD 128) or 32-byte (64) pieces exchanged by the pair's number so that the
 //      lanes of a load, which hold four pairs each, meet no bank twice.
 #pragma once
+#include <type_traits>
+
 #include "fb_common.cuh"
 
 namespace fb {
@@ -203,36 +205,43 @@ __global__ void __launch_bounds__(256) kv4_read(const Kv4Read P) {
   const int m = blockIdx.x, lane = threadIdx.x & 31;
   pdl_begin(true);
   const int b = kv4_seq_of(S, m, lane);
-  if (b < 0) return;
   Kv4Seq q;
-  if (!q.get(S, b, threadIdx.x == 0) || m < q.first || m >= q.first + q.n) return;
-  const int slot = q.cached + m - q.first, page = kv4_page(S, b, slot, threadIdx.x == 0), p = slot & 15;
-  if (page < 0 || lane >= HD / 4) return;
+  int page = -1, slot = 0;
+  if (b >= 0 && q.get(S, b, threadIdx.x == 0) && m >= q.first && m < q.first + q.n) {
+    slot = q.cached + m - q.first;
+    page = kv4_page(S, b, slot, threadIdx.x == 0);
+  }
+  const int p = slot & 15;
+  if (lane >= HD / 4) return;
   for (int r = threadIdx.x >> 5; r < 2 * S.nkv; r += 8) {
     const bool isv = r >= S.nkv;
     const int head = isv ? r - S.nkv : r;
     float* out = isv ? P.v : P.k;
     if (!out) continue;
-    const uint8_t* blk = kv4_block<HD>(S, page, head, slot) + blockIdx.y * P.layer;
-    const uint32_t sz = *reinterpret_cast<const uint32_t*>(blk + (isv ? C::VSZ : C::KSZ) + p * 4);
-    float x[4];
-    if (isv) {
-      const uint32_t h = *reinterpret_cast<const uint16_t*>(blk + C::v_word(p >> 1, lane) + (p & 1) * 2);
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (page >= 0) {
+      const uint8_t* blk = kv4_block<HD>(S, page, head, slot) + blockIdx.y * P.layer;
+      const uint32_t sz = *reinterpret_cast<const uint32_t*>(blk + (isv ? C::VSZ : C::KSZ) + p * 4);
+      if (isv) {
+        const uint32_t h = *reinterpret_cast<const uint16_t*>(blk + C::v_word(p >> 1, lane) + (p & 1) * 2);
 #pragma unroll
-      for (int e = 0; e < 4; e++) x[e] = (float)((int)(h >> (4 * e) & 15u) - 8);
-    } else {
-      const uint32_t h = *reinterpret_cast<const uint32_t*>(blk + C::k_word(p, lane >> 1)) >> (8 * (lane & 1));
+        for (int e = 0; e < 4; e++) x[e] = (float)((int)(h >> (4 * e) & 15u) - 8);
+      } else {
+        const uint32_t h = *reinterpret_cast<const uint32_t*>(blk + C::k_word(p, lane >> 1)) >> (8 * (lane & 1));
 #pragma unroll
-      for (int e = 0; e < 4; e++) x[e] = (float)((int)(h >> ((e & 1) * 16 + (e >> 1) * 4) & 15u) - 8);
+        for (int e = 0; e < 4; e++) x[e] = (float)((int)(h >> ((e & 1) * 16 + (e >> 1) * 4) & 15u) - 8);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = __fadd_rn(__fmul_rn(x[e], bflo(sz)), bfhi(sz));
     }
-#pragma unroll
-    for (int e = 0; e < 4; e++) x[e] = __fadd_rn(__fmul_rn(x[e], bflo(sz)), bfhi(sz));
     *reinterpret_cast<float4*>(out + (((size_t)blockIdx.y * S.T + m) * S.nkv + head) * HD + 4 * lane) = make_float4(x[0], x[1], x[2], x[3]);
   }
 }
 
 // Rows of a sequence from slots to slots, in order, in every layer. A thread owns the same piece of every row (a word of K, a half of V, a pair), so that a
-// move that reads what an earlier one wrote finds it written without a wait between threads. grid (nkv, layers), 128 threads.
+// move that reads what an earlier one wrote finds it written without a wait between threads. An accepted path never does (its rows lie behind the places that
+// they go to), and then eight loads are under way side by side. grid (nkv, layers), 128 threads. Bound by latency: the path, the pages, the
+// rows, one after the other.
 struct Kv4Move {
   Kv4Seqs S;
   size_t layer;
@@ -244,29 +253,21 @@ struct Kv4Move {
 template <int HD>
 __global__ void __launch_bounds__(128) kv4_move(const Kv4Move P) {
   using C = Kv4<HD>;
-  constexpr int KW = HD / 8, VH = HD / 4;
+  constexpr int KW = HD / 8, VH = HD / 4, N = 64;
   static_assert(KW + VH + 2 <= 128, "a thread per piece of a row");
+  __shared__ int s_from[N], s_to[N], s_page_from[N], s_page_to[N];
   const Kv4Seqs& S = P.S;
   const int tid = threadIdx.x, head = blockIdx.x;
-  const bool first = tid == 0 && head == 0 && blockIdx.y == 0;
+  const bool first = head == 0 && blockIdx.y == 0;
   pdl_begin(true);
   int len = P.n;
   if (P.accept) {
     len = P.accept[0];
     if (len < 0 || len > P.most) {
-      if (first) kv4_report(S.status, KV4_PATH, 0, P.most, len);
+      if (first && tid == 0) kv4_report(S.status, KV4_PATH, 0, P.most, len);
       return;
     }
   }
-  auto slots = [&](int i, int& from, int& to) {
-    if (!P.accept) { from = P.src[i]; to = P.dst[i]; return true; }
-    const int node = P.accept[2 + i];
-    from = P.pos + node;
-    to = P.pos + i;
-    if (node >= 0 && (long long)P.pos + node < (long long)S.table_ld * kPage && to < S.table_ld * kPage) return true;
-    if (first) kv4_report(S.status, KV4_PATH, i, S.table_ld * kPage, node);
-    return false;
-  };
   uint8_t* pool = S.pool + blockIdx.y * P.layer;
   auto at = [&](int page, int slot) {
     uint8_t* blk = pool + ((size_t)page * S.nkv + head) * C::REC + (slot % kPage / 16) * C::BLOCK;
@@ -275,22 +276,58 @@ __global__ void __launch_bounds__(128) kv4_move(const Kv4Move P) {
     if (tid < KW + VH) return blk + C::v_word(p >> 1, tid - KW) + (p & 1) * 2;
     return blk + (tid == KW + VH ? C::KSZ : C::VSZ) + p * 4;
   };
-  const bool half = tid >= KW && tid < KW + VH;
-  for (int i = P.accept ? 1 : 0; i < len; i++) {
-    int from, to;
-    if (!slots(i, from, to) || from == to) continue;
-    const int pf = kv4_page(S, 0, from, first), pt = kv4_page(S, 0, to, first);
-    if (pf < 0 || pt < 0 || tid >= KW + VH + 2) continue;
-    const uint8_t* a = at(pf, from);
-    uint8_t* d = at(pt, to);
-    if (half) *reinterpret_cast<uint16_t*>(d) = *reinterpret_cast<const volatile uint16_t*>(a);
-    else *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const volatile uint32_t*>(a);
+  const bool half = tid >= KW && tid < KW + VH, piece = tid < KW + VH + 2;
+  auto load = [&](int i) -> uint32_t {
+    const uint8_t* a = at(s_page_from[i], s_from[i]);
+    return half ? *reinterpret_cast<const volatile uint16_t*>(a) : *reinterpret_cast<const volatile uint32_t*>(a);
+  };
+  auto store = [&](int i, uint32_t v) {
+    uint8_t* d = at(s_page_to[i], s_to[i]);
+    if (half) *reinterpret_cast<volatile uint16_t*>(d) = (uint16_t)v;
+    else *reinterpret_cast<volatile uint32_t*>(d) = v;
+  };
+  for (int i0 = P.accept ? 1 : 0; i0 < len; i0 += N) {           // the same for all threads
+    const int n = min(N, len - i0);
+    bool chain = false;
+    if (tid < n) {
+      int from, to;
+      bool ok = true;
+      if (P.accept) {
+        const int node = P.accept[2 + i0 + tid];
+        ok = node >= 0 && (long long)P.pos + node < (long long)S.table_ld * kPage && (long long)P.pos + i0 + tid < (long long)S.table_ld * kPage;
+        if (!ok && first) kv4_report(S.status, KV4_PATH, i0 + tid, S.table_ld * kPage, node);
+        from = P.pos + node;
+        to = P.pos + i0 + tid;
+        chain = from < to;
+      } else {
+        from = P.src[tid];
+        to = P.dst[tid];
+        chain = true;
+      }
+      const int pf = ok && from != to ? kv4_page(S, 0, from, first) : -1, pt = pf >= 0 ? kv4_page(S, 0, to, first) : -1;
+      s_from[tid] = from; s_to[tid] = to; s_page_from[tid] = pt >= 0 ? pf : -1; s_page_to[tid] = pt;
+    }
+    if (__syncthreads_or(chain)) {
+      for (int i = 0; i < n && piece; i++)
+        if (s_page_from[i] >= 0) store(i, load(i));
+    } else {
+      for (int i = 0; i < n && piece; i += 8) {
+        uint32_t v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = i + k < n && s_page_from[i + k] >= 0 ? load(i + k) : 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          if (i + k < n && s_page_from[i + k] >= 0) store(i + k, v[k]);
+      }
+    }
+    __syncthreads();
   }
 }
 
 // ------------------------------------------------------------------------------------------------ attention, few rows
+// (not volatile: independent products may pass one another)
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -304,111 +341,246 @@ __device__ __forceinline__ uint32_t cvt_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
-// nibble pairs in bits (0..3, 16..19) / (4..7, 20..23) -> fp16 pair nib - 8, exact (fb_vtc.cuh's conversion without the scale)
-__device__ __forceinline__ uint32_t kv4_lo(uint32_t w) {
-  const uint32_t x = (w & 0x000F000Fu) | 0x64006400u;
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6408)));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t kv4_hi(uint32_t w) {
-  const uint32_t x = (w & 0x00F000F0u) | 0x64006400u;
-  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x2C00)), __half2half2(__ushort_as_half(0xD480)));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint32_t kv4_lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-
 struct Kv4Attend {
   Kv4Seqs S;
   const uint16_t* q;         // bf16 [T][nh][HD], rotated, tokens q_ld elements apart
   uint16_t* out;             // bf16 [T][nh][HD], tokens o_ld apart
   long long q_ld, o_ld;
   const uint8_t* amask;      // [T][mask_ld]: token m sees new slot j of its sequence, or nullptr: causal
-  int mask_ld, nh, R, max_new, groups, nsplit;
+  int mask_ld, nh, R;
+  int nsplit;                // a cluster: its CTAs share the positions of a row group of the one sequence
+  int slots, chunk;          // else: CTAs that the GPU holds, over which all positions are spread in pieces of `chunk` units or more; slots 0: whole
+  float* work;               // partials of split row groups, [task][row][PW], for kv4_join
   float scale;               // times log2(e)
   unsigned spin_limit;
 };
 
+// What a CTA does: `n` units from `unit` on of the positions that query rows r0 .. of a sequence and kv head see; `parts` tasks share them, the first of
+// them is task `first`. The lengths are the device's, so every CTA finds its own task: per = all units of all row groups / slots, a sequence's
+// parts follow from that, and the task's sequence from the sum of the tasks ahead of it. A ragged batch is spread evenly whatever its lengths.
+template <int ROWS, int U>
+struct Kv4Task {
+  Kv4Seq seq;
+  int b, kvh, rows, r0, total, unit, n, parts;
+  long long first;
+  __device__ __forceinline__ int groups_of(const Kv4Attend& P, const Kv4Seq& q) const { return (int)(((long long)q.n * P.R + ROWS - 1) / ROWS); }
+  __device__ __forceinline__ int units_of(const Kv4Seq& q) const { return (int)(((long long)q.cached + q.n + U - 1) / U); }
+  __device__ __forceinline__ int parts_of(int units, int per) const { return (units - 1) / per + 1; }        // per may be the largest integer
+  // group grp of the sequence in `seq`
+  __device__ __forceinline__ int set(const Kv4Attend& P, int grp) {          // units that the group sees
+    rows = seq.n * P.R;
+    r0 = grp * ROWS;
+    total = seq.cached + seq.n;
+    const int t_end = P.amask ? total : seq.cached + min(seq.n - 1, (r0 + ROWS - 1) / P.R) + 1;
+    return (t_end + U - 1) / U;
+  }
+  __device__ __forceinline__ int per_of(const Kv4Attend& P, long long units) const {
+    if (!P.slots) return 0x7fffffff;
+    const long long per = (units * P.S.nkv + P.slots - 1) / P.slots;
+    return (int)min(max(per, (long long)P.chunk), 0x7fffffffll);
+  }
+  // task `idx`, or with JOIN row group `idx` of all sequences, all of its parts
+  template <bool JOIN>
+  __device__ __forceinline__ bool find(const Kv4Attend& P, long long idx, int lane, bool report) {
+    const Kv4Seqs& S = P.S;
+    int per, g = 0, part = 0;
+    if (S.n_seq == 1) {
+      b = 0;
+      if (!seq.get(S, 0, report)) return false;
+      const int groups = groups_of(P, seq), nu = units_of(seq);
+      per = per_of(P, (long long)groups * nu);
+      parts = parts_of(nu, per);
+      first = 0;
+      if (JOIN) {
+        g = (int)idx;
+        if (g >= groups) return false;
+      } else {
+        if (idx >= (long long)groups * parts * S.nkv) return false;
+      }
+    } else {
+      long long units = 0;
+      for (int i = lane; i < S.n_seq; i += 32) {
+        Kv4Seq q;
+        if (q.get(S, i, report)) units += (long long)groups_of(P, q) * units_of(q);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
+      per = per_of(P, units);
+      long long at = 0, tasks_ahead = 0;                         // what is counted (tasks, or row groups), and tasks, ahead of the 32 sequences
+      int i0 = 0;
+      for (;; i0 += 32) {
+        if (i0 >= S.n_seq) return false;
+        Kv4Seq q;
+        long long tasks = 0, count = 0;
+        if (i0 + lane < S.n_seq && q.get(S, i0 + lane, false)) {
+          const int groups = groups_of(P, q), nu = units_of(q);
+          tasks = (long long)groups * parts_of(nu, per) * S.nkv;
+          count = JOIN ? groups : tasks;
+        }
+        long long sum = count, tsum = tasks;                     // inclusive sums over the lanes
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+          const long long x = __shfl_up_sync(0xffffffffu, sum, o), y = __shfl_up_sync(0xffffffffu, tsum, o);
+          if (lane >= o) { sum += x; tsum += y; }
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, idx < at + sum);
+        if (past) {
+          const int l = __ffs(past) - 1;
+          b = i0 + l;
+          idx -= at + __shfl_sync(0xffffffffu, sum - count, l);
+          first = tasks_ahead + __shfl_sync(0xffffffffu, tsum - tasks, l);
+          break;
+        }
+        at += __shfl_sync(0xffffffffu, sum, 31);
+        tasks_ahead += __shfl_sync(0xffffffffu, tsum, 31);
+      }
+      seq.get(S, b, false);
+      parts = parts_of(units_of(seq), per);
+      g = (int)idx;
+    }
+    if (!JOIN) {                                                 // a sequence's tasks: parts, row groups, kv heads
+      const int groups = groups_of(P, seq), i = (int)(idx / S.nkv);
+      kvh = (int)(idx % S.nkv);
+      part = i / groups;
+      g = i % groups;
+    }
+    const int nu = set(P, g);
+    unit = (int)min((long long)part * per, (long long)nu);       // a causal group may see less than the sequence's parts cover: it has empty ones
+    n = (int)min((long long)per, (long long)nu - unit);
+    return true;
+  }
+  __device__ __forceinline__ long long task_of(const Kv4Attend& P, int part) const {       // part `part` of this row group and kv head
+    return first + ((long long)part * groups_of(P, seq) + r0 / ROWS) * P.S.nkv + kvh;
+  }
+};
+
+// Partials of a row, n of them `stride` floats apart, eight loads side by side: lane < HD / 4 merges dims 4 lane .. 4 lane + 3
+template <int HD>
+__device__ __forceinline__ void kv4_merge(const float* p0, int n, size_t stride, int lane, float4& acc, float& mm, float& den) {
+  mm = -1e30f;
+  den = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += 8) {
+    float2 ml[8];
+    float4 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const float* p = p0 + (i0 + k < n ? i0 + k : i0) * stride;
+      ml[k] = *reinterpret_cast<const float2*>(p + HD);
+      v[k] = lane < HD / 4 ? *reinterpret_cast<const float4*>(p + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i0 + k >= n) ml[k].x = -INFINITY;
+    }
+    float top = mm;
+#pragma unroll
+    for (int k = 0; k < 8; k++) top = fmaxf(top, ml[k].x);
+    const float old = ex2(mm - top);
+    mm = top;
+    den *= old;
+    acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      if (i0 + k < n) {
+        const float e = ex2(ml[k].x - mm);
+        den = fmaf(ml[k].y, e, den);
+        acc.x = fmaf(v[k].x, e, acc.x); acc.y = fmaf(v[k].y, e, acc.y); acc.z = fmaf(v[k].z, e, acc.z); acc.w = fmaf(v[k].w, e, acc.w);
+      }
+    }
+  }
+}
+// normalise and write row r of a sequence; a row that sees nothing is zeros
+template <int HD>
+__device__ __forceinline__ void kv4_finish(const Kv4Attend& P, const Kv4Seq& seq, int kvh, int r, int lane, const float4& acc, float den) {
+  if (lane >= HD / 4) return;
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  *reinterpret_cast<uint2*>(P.out + (size_t)(seq.first + r / P.R) * P.o_ld + (size_t)(kvh * P.R + r % P.R) * HD + lane * 4) =
+      make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+}
+
 // Scores and outputs are computed TRANSPOSED: S^T[16 positions][8 query rows] = K Q^T and O^T[16 dims][8 query rows] += V^T P^T by mma.m16n8k16, so that
 // the few query rows of a decode step (row = token * R + head of the group) fill the narrow side of the instruction and the cache the wide one. The cache's
-// operands are nib - 8 in fp16, exact; a position's s and z join in fp32 behind the product, S = s (q . n) + z (sum q), and ahead of it,
-// O += (p s) n, and sum p z apart. Q is fp16 times a power of two per row (exact for elements down to 2^-31 of the row's largest); p s is rounded to
-// fp16 (half a step is 2^-11 of it, the output's bf16 rounding 2^-8), times a power of two that follows the largest p s of the row so far.
-// A warp streams units of U positions through a ring of its own, one bulk copy each (lane 0 asks, all 32 lanes read), with a running maximum and sum;
-// warps meet at the end, then the CTAs of a cluster that share a sequence's positions (partials pushed to the CTA that finishes the row).
+// operands are its nibbles as they lie, masked: nib 2^-24 and 16 nib 2^-24, subnormal fp16 numbers, which the tensor pipe multiplies exactly; the 16 is
+// taken out of Q for the keys and of the outputs for the values. A position's s and z join in fp32, S = s (q . nib) + (z - 8 s) (sum q) behind the product, and
+// (p s) ahead of it for O, with the sum of p (z - 8 s) apart. Q is fp16 times a power of two per row (exact for elements down to 2^-27 of the row's
+// largest); p s is rounded to fp16 (half a step is 2^-11 of it, the output's bf16 rounding 2^-8) times a power of two that follows the row's largest p s.
+// The maximum that p refers to and that power are looked at by votes and moved only when a score is more than 2^6 above the one or a p s 2^14 above the other.
+// Warps 0 .. W-1 take the CTA's units of U positions in turn, each through NST stages of its own; lane w of warp W brings the units of warp w, one bulk copy
+// each. They meet at the end, then the CTAs that share the positions: a cluster pushes its partials to the CTA that finishes the row, more CTAs
+// than a cluster leave them to kv4_join.
 template <int HD, int NQ, int W>
 struct Kv4Few {
   static constexpr int U = 32, NST = 3, ROWS = 8 * NQ, PW = HD + 4;         // positions of a unit, stages of a warp, query rows, floats of a partial
   static constexpr int STAGE = U / 16 * Kv4<HD>::BLOCK, RING = W * NST * STAGE, PART = W * ROWS * PW * 4;
   static constexpr int INBOX = RING > PART ? RING : PART;
-  static constexpr int BAR = INBOX + 16 * PW * 4, TOTAL = BAR + W * NST * 8 + 16;
-  static_assert(TOTAL <= 227 * 1024, "shared memory");
+  static constexpr int BAR = INBOX + 16 * PW * 4, SKIP = BAR + 2 * W * NST * 8, TOTAL = SKIP + W * NST * 4 + 16;
+  static_assert(TOTAL <= 227 * 1024 && W < 32, "shared memory, a lane per warp");
 };
 
-// grid (clusters of nsplit over sequence x row group, nkv), W warps
-template <int HD, int NQ, int W>
-__global__ void __launch_bounds__(W * 32) kv4_attn_few(const Kv4Attend P) {
+// W + 1 warps. CLUSTER: grid (nsplit x row groups, nkv) of one sequence, the nsplit CTAs are a cluster; else grid (tasks)
+template <int HD, int NQ, int W, bool CLUSTER>
+__global__ void __launch_bounds__(W * 32 + 32) kv4_attn_few(const Kv4Attend P) {
   using C = Kv4<HD>;
   using F = Kv4Few<HD, NQ, W>;
-  constexpr int KS = HD / 16, MT = HD / 16, U = F::U, NST = F::NST, ROWS = F::ROWS, PW = F::PW;
+  constexpr int KS = HD / 16, MT = HD / 16, NW = HD / 32 + (HD > C::MAIN), U = F::U, NST = F::NST, ROWS = F::ROWS, PW = F::PW;
   extern __shared__ __align__(128) uint8_t sm[];
   const Kv4Seqs& S = P.S;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int ns = P.nsplit, rank = (int)blockIdx.x % ns, idx = (int)blockIdx.x / ns, b = idx / P.groups, grp = idx % P.groups, kvh = blockIdx.y, R = P.R;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + F::BAR) + warp * NST;
-  volatile int* s_abort = reinterpret_cast<volatile int*>(sm + F::BAR + W * NST * 8);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, R = P.R;
+  uint64_t *full = reinterpret_cast<uint64_t*>(sm + F::BAR), *empty = full + W * NST;      // [stage][warp]
+  volatile int* s_skip = reinterpret_cast<volatile int*>(sm + F::SKIP);                     // the stage's unit has no page
+  volatile int* s_abort = s_skip + W * NST;
   pdl_begin(true);
-  Kv4Seq seq;
-  const bool told = kvh == 0 && rank == 0 && grp == 0 && tid == 0;
-  if (!seq.get(S, b, told)) return;                              // the same for every CTA of a cluster
-  if (told && seq.n > P.max_new) kv4_report(S.status, KV4_TOKENS, b, P.max_new, seq.n);
-  const int rows = seq.n * R, r0 = grp * ROWS;
-  if (r0 >= rows) return;
-  if (ns > 1) cluster_arrive();                                  // partials are sent once every neighbour is known to run
-  if (lane == 0) {
-    for (int i = 0; i < NST; i++) mbar_init(&bars[i], 1);
-    if (warp == 0) *s_abort = 0;
+  Kv4Task<ROWS, U> task;
+  const int ns = CLUSTER ? P.nsplit : 1, rank = CLUSTER ? (int)blockIdx.x % ns : 0;
+  if (CLUSTER) {
+    task.b = 0;
+    task.kvh = blockIdx.y;
+    if (!task.seq.get(S, 0, blockIdx.x == 0 && blockIdx.y == 0 && tid == 0)) return;         // the same for every CTA of a cluster
+    const int grp = (int)blockIdx.x / ns, nu = task.set(P, grp), per = (nu + ns - 1) / ns;
+    task.unit = min(rank * per, nu);
+    task.n = min(per, nu - task.unit);
+  } else if (!task.template find<false>(P, blockIdx.x, lane, blockIdx.x == 0 && warp == 0)) {
+    return;
+  }
+  const Kv4Seq& seq = task.seq;
+  const int rows = task.rows, r0 = task.r0, total = task.total, kvh = task.kvh, b = task.b;
+  if (CLUSTER) cluster_arrive();                                 // partials are sent once every neighbour is known to run
+  const int u_begin = task.unit, n = task.n, rounds = (n + W - 1) / W;
+  int page = warp == W && lane < min(W, n) ? kv4_page(S, b, (u_begin + lane) * U, true) : -1;
+  if (tid < W * NST) {
+    mbar_init(&full[tid], 1);
+    mbar_init(&empty[tid], 1);
     mbar_fence_init();
   }
+  if (tid == 0) *s_abort = 0;
   __syncthreads();
   const WaitCtl wc{S.status, s_abort, P.spin_limit};
-  const int m_last = min(seq.n - 1, (r0 + ROWS - 1) / R), total = seq.cached + seq.n, t_end = P.amask ? total : seq.cached + m_last + 1;
-  const int nu = (t_end + U - 1) / U, u_begin = (int)((long long)nu * rank / ns), u_end = (int)((long long)nu * (rank + 1) / ns);
-  const int mine = u_end - u_begin > warp ? (u_end - u_begin - warp + W - 1) / W : 0;      // units of this warp: u_begin + warp + i * W
-  uint32_t skip = 0;                                             // stages whose unit has no page
-  uint8_t* ring = sm + warp * NST * F::STAGE;
-  auto page_of = [&](int i) { return i < mine ? kv4_page(S, b, (u_begin + warp + i * W) * U, lane == 0) : -1; };
-  auto issue = [&](int i, int page, int st) {
-    if (i >= mine) return;
-    if (page < 0) {
-      skip |= 1u << st;
-      if (lane == 0) mbar_arrive(&bars[st]);
-      return;
+  bool ok = true;
+  int issued = 0;                                                // rounds that the copying warp has begun
+  if (warp == W) {
+    int st = 0;
+    uint32_t lap = 1;
+    for (; issued < rounds && ok; issued++) {
+      const int i = issued * W + lane;
+      const bool mine = lane < W && i < n;
+      const int now = page;
+      if (mine && i + W < n) page = kv4_page(S, b, (u_begin + i + W) * U, true);
+      if (mine) {
+        const int k = st * W + lane;
+        ok = mbar_wait(&empty[k], lap, wc, W_EMPTY, 31);
+        if (ok) {
+          s_skip[k] = now < 0;
+          if (now < 0) {
+            mbar_arrive(&full[k]);
+          } else {
+            mbar_expect_tx(&full[k], F::STAGE);
+            bulk_g2s(sm + k * F::STAGE, kv4_block<HD>(S, now, kvh, (u_begin + i) * U), F::STAGE, &full[k]);
+          }
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (++st == NST) { st = 0; lap ^= 1u; }
     }
-    skip &= ~(1u << st);
-    if (lane == 0) {
-      const int slot = (u_begin + warp + i * W) * U;
-      mbar_expect_tx(&bars[st], F::STAGE);
-      bulk_g2s(ring + st * F::STAGE, kv4_block<HD>(S, page, kvh, slot), F::STAGE, &bars[st]);
-    }
-  };
-  {
-    int pg[NST];
-#pragma unroll
-    for (int i = 0; i < NST; i++) pg[i] = page_of(i);
-#pragma unroll
-    for (int i = 0; i < NST; i++) issue(i, pg[i], i);
   }
-  int page_next = page_of(NST);
-
   // the query rows: lane (g, t) holds row g of each tile, the dims that it multiplies
   uint32_t qf[NQ][KS][2];
   float c2[NQ][2], qs[NQ][2];                                    // of columns 2t, 2t + 1: factor of the scores, sum of the row
@@ -437,185 +609,215 @@ __global__ void __launch_bounds__(W * 32) kv4_attn_few(const Kv4Attend P) {
     const float2 f = pow2_for(mx);
 #pragma unroll
     for (int i = 0; i < 2 * KS; i++) {
-      const float a = bflo(w[i]) * f.x, c = bfhi(w[i]) * f.x;
+      const float a = bflo(w[i]) * f.x, c = bfhi(w[i]) * f.x, h = i & 1 ? 0.0625f : 1.f;
       sum += a + c;
-      qf[nq][i >> 1][i & 1] = cvt_f16x2(a, c);
+      qf[nq][i >> 1][i & 1] = cvt_f16x2(a * h, c * h);
     }
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-      c2[nq][e] = __shfl_sync(0xffffffffu, f.y, (2 * t + e) * 4) * P.scale;
-      qs[nq][e] = __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4);
+      c2[nq][e] = __shfl_sync(0xffffffffu, f.y, (2 * t + e) * 4) * P.scale * 0x1p24f;
+      qs[nq][e] = __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4) * 0x1p-24f;
     }
   }
-  float o[NQ][MT][4], mrun[NQ][2], lrun[NQ][2], zrun[NQ][2], wrun[NQ][2];
-  uint32_t erun[NQ][2];                                          // exponent field of wrun, the largest p s so far: o is in units of 2^(erun - 127)
+  float o[NQ][MT][4], mrun[NQ][2], lrun[NQ][2], zrun[NQ][2];
+  float wtop[NQ][2], wlim[NQ][2], vf[NQ][2];                     // this lane's largest p s, how large one may be, the power of two that p s is multiplied by:
+  uint32_t erun[NQ][2];                                          // 2^(127 - erun), o is in units of its inverse (and of 2^-24 or 2^-20)
 #pragma unroll
   for (int nq = 0; nq < NQ; nq++) {
 #pragma unroll
     for (int i = 0; i < MT; i++) o[nq][i][0] = o[nq][i][1] = o[nq][i][2] = o[nq][i][3] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 2; e++) { mrun[nq][e] = -1e30f; lrun[nq][e] = 0.f; zrun[nq][e] = 0.f; wrun[nq][e] = 0.f; erun[nq][e] = 1; }
+    for (int e = 0; e < 2; e++) {
+      mrun[nq][e] = -1e30f; lrun[nq][e] = 0.f; zrun[nq][e] = 0.f;
+      wtop[nq][e] = 0.f; wlim[nq][e] = 0.f; vf[nq][e] = 1.f; erun[nq][e] = 127;
+    }
   }
-  bool ok = true;
-  int st = 0;
-  uint32_t lap = 0;
-  int done = 0;
-#pragma unroll 1
-  for (int i = 0; i < mine; i++) {
-    ok = __all_sync(0xffffffffu, mbar_wait(&bars[st], lap, wc, W_FULL, 30));
-    if (!ok) break;
-    done = i + 1;
-    const int slot0 = (u_begin + warp + i * W) * U;
-    if (!(skip >> st & 1)) {
-      const uint32_t base = smem_u32(ring + st * F::STAGE);
-      const bool edge = slot0 + U > seq.cached;                  // holds new tokens, or slots behind them
-      float sc[NQ][U / 16][4], vs[U / 16][2], vz[U / 16][2];
+  auto scale_o = [&](int nq, float a, float c) {
 #pragma unroll
-      for (int k = 0; k < U / 16; k++) {
-        const uint32_t blk = base + k * C::BLOCK;
+    for (int j = 0; j < MT; j++) { o[nq][j][0] *= a; o[nq][j][1] *= c; o[nq][j][2] *= a; o[nq][j][3] *= c; }
+  };
+  auto top = [&](float x) {                                      // over the lanes of a column
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+    return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+  };
+  // one unit; EDGE: it holds new tokens, or slots behind them
+  auto unit = [&](const uint8_t* base, int slot0, auto edge) {
+    constexpr bool EDGE = decltype(edge)::value;
+    float sc[NQ][U / 16][4], vs[U / 16][2], vz[U / 16][2];
+    uint32_t unseen[NQ];                                         // EDGE: bit 4 k + i: element i of block k is not seen
 #pragma unroll
-        for (int nq = 0; nq < NQ; nq++) sc[nq][k][0] = sc[nq][k][1] = sc[nq][k][2] = sc[nq][k][3] = 0.f;
-        uint32_t wl[HD / 32 + (HD > C::MAIN)], wh[HD / 32 + (HD > C::MAIN)];       // words of positions g and g + 8
-        if constexpr (HD == 128) {
-          const uint4 x = lds128(blk + g * 64 + t * 16), y = lds128(blk + (g + 8) * 64 + t * 16);
-          wl[0] = x.x; wl[1] = x.y; wl[2] = x.z; wl[3] = x.w;
-          wh[0] = y.x; wh[1] = y.y; wh[2] = y.z; wh[3] = y.w;
-        } else {
-          const uint2 x = lds64(blk + g * 32 + t * 8), y = lds64(blk + (g + 8) * 32 + t * 8);
-          wl[0] = x.x; wl[1] = x.y;
-          wh[0] = y.x; wh[1] = y.y;
-          if constexpr (HD > C::MAIN) {
-            wl[2] = kv4_lds32(blk + 512 + g * 8 + (t >> 1) * 4) >> (8 * (t & 1));
-            wh[2] = kv4_lds32(blk + 512 + (g + 8) * 8 + (t >> 1) * 4) >> (8 * (t & 1));
-          }
-        }
+    for (int nq = 0; nq < NQ; nq++) unseen[nq] = 0;
+    uint32_t wl[U / 16][NW], wh[U / 16][NW];                     // words of positions g and g + 8
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-          const uint32_t a = wl[ks >> 1] >> (8 * (ks & 1)), c = wh[ks >> 1] >> (8 * (ks & 1));
-          const uint32_t A[4] = {kv4_lo(a), kv4_lo(c), kv4_hi(a), kv4_hi(c)};
+    for (int k = 0; k < U / 16; k++) {
+      const uint8_t* blk = base + k * C::BLOCK;
 #pragma unroll
-          for (int nq = 0; nq < NQ; nq++) mma_f16(sc[nq][k], A, qf[nq][ks][0], qf[nq][ks][1]);
-        }
-        const uint32_t k0 = kv4_lds32(blk + C::KSZ + g * 4), k1 = kv4_lds32(blk + C::KSZ + g * 4 + 32), v0 = kv4_lds32(blk + C::VSZ + g * 4),
-                       v1 = kv4_lds32(blk + C::VSZ + g * 4 + 32);
-        vs[k][0] = bflo(v0); vs[k][1] = bflo(v1); vz[k][0] = bfhi(v0); vz[k][1] = bfhi(v1);
-        const float s0 = bflo(k0), s1 = bflo(k1), z0 = bfhi(k0), z1 = bfhi(k1);
-#pragma unroll
-        for (int nq = 0; nq < NQ; nq++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) sc[nq][k][e] = fmaf(e < 2 ? z0 : z1, qs[nq][e & 1], sc[nq][k][e] * (e < 2 ? s0 : s1)) * c2[nq][e & 1];
-        if (edge) {
-#pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const int tp = slot0 + k * 16 + g + 8 * h;
-            if (tp >= total) vs[k][h] = vz[k][h] = 0.f;          // what lies behind the last token may be anything
-#pragma unroll
-            for (int nq = 0; nq < NQ; nq++)
-#pragma unroll
-              for (int e = 0; e < 2; e++) {
-                bool see = tp < total;
-                if (see && tp >= seq.cached) {
-                  const int mq = min(r0 + nq * 8 + 2 * t + e, rows - 1) / R, j = tp - seq.cached;
-                  see = P.amask ? j < P.mask_ld && P.amask[(size_t)(seq.first + mq) * P.mask_ld + j] != 0 : j <= mq;
-                }
-                if (!see) sc[nq][k][2 * h + e] = -INFINITY;
-              }
-          }
+      for (int nq = 0; nq < NQ; nq++) sc[nq][k][0] = sc[nq][k][1] = sc[nq][k][2] = sc[nq][k][3] = 0.f;
+      if constexpr (HD == 128) {
+        const uint4 x = *reinterpret_cast<const uint4*>(blk + g * 64 + t * 16), y = *reinterpret_cast<const uint4*>(blk + (g + 8) * 64 + t * 16);
+        wl[k][0] = x.x; wl[k][1] = x.y; wl[k][2] = x.z; wl[k][3] = x.w;
+        wh[k][0] = y.x; wh[k][1] = y.y; wh[k][2] = y.z; wh[k][3] = y.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(blk + g * 32 + t * 8), y = *reinterpret_cast<const uint2*>(blk + (g + 8) * 32 + t * 8);
+        wl[k][0] = x.x; wl[k][1] = x.y;
+        wh[k][0] = y.x; wh[k][1] = y.y;
+        if constexpr (HD > C::MAIN) {
+          wl[k][2] = *reinterpret_cast<const uint32_t*>(blk + 512 + g * 8 + (t >> 1) * 4) >> (8 * (t & 1));
+          wh[k][2] = *reinterpret_cast<const uint32_t*>(blk + 512 + (g + 8) * 8 + (t >> 1) * 4) >> (8 * (t & 1));
         }
       }
-      // running maximum, sums, and p s in place of the scores
-      float corr[NQ][2];
-      bool moved = false;
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+      for (int k = 0; k < U / 16; k++) {
+        const uint32_t a = wl[k][ks >> 1] >> (8 * (ks & 1)), c = wh[k][ks >> 1] >> (8 * (ks & 1));
+        const uint32_t A[4] = {a & 0x000F000Fu, c & 0x000F000Fu, a & 0x00F000F0u, c & 0x00F000F0u};
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) mma_f16(sc[nq][k], A, qf[nq][ks][0], qf[nq][ks][1]);
+      }
+#pragma unroll
+    for (int k = 0; k < U / 16; k++) {
+      const uint8_t* blk = base + k * C::BLOCK;
+      auto pair = [&](int off) { return *reinterpret_cast<const uint32_t*>(blk + off + g * 4); };
+      const uint32_t k0 = pair(C::KSZ), k1 = pair(C::KSZ + 32), v0 = pair(C::VSZ), v1 = pair(C::VSZ + 32);
+      vs[k][0] = bflo(v0); vs[k][1] = bflo(v1); vz[k][0] = fmaf(-8.f, vs[k][0], bfhi(v0)); vz[k][1] = fmaf(-8.f, vs[k][1], bfhi(v1));
+      const float s0 = bflo(k0), s1 = bflo(k1), z0 = fmaf(-8.f, s0, bfhi(k0)), z1 = fmaf(-8.f, s1, bfhi(k1));
 #pragma unroll
       for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) sc[nq][k][e] = fmaf(e < 2 ? z0 : z1, qs[nq][e & 1], sc[nq][k][e] * (e < 2 ? s0 : s1)) * c2[nq][e & 1];
+      if (EDGE) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int tp = slot0 + k * 16 + g + 8 * h, j = tp - seq.cached;
+#pragma unroll
+          for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              bool see = tp < total;
+              if (see && j >= 0) {
+                const int mq = min(r0 + nq * 8 + 2 * t + e, rows - 1) / R;
+                see = P.amask ? j < P.mask_ld && P.amask[(size_t)(seq.first + mq) * P.mask_ld + j] != 0 : j <= mq;
+              }
+              if (!see) { sc[nq][k][2 * h + e] = -INFINITY; unseen[nq] |= 1u << (4 * k + 2 * h + e); }
+            }
+        }
+      }
+    }
+    bool far = false;
+#pragma unroll
+    for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int k = 0; k < U / 16; k++) far = far || fmaxf(sc[nq][k][e], sc[nq][k][2 + e]) > mrun[nq][e] + 6.f;
+    const bool moved = __any_sync(0xffffffffu, far);
+    if (moved) {
+#pragma unroll
+      for (int nq = 0; nq < NQ; nq++) {
+        float cr[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           float mx = -INFINITY;
 #pragma unroll
           for (int k = 0; k < U / 16; k++) mx = fmaxf(mx, fmaxf(sc[nq][k][e], sc[nq][k][2 + e]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const float mn = fmaxf(mrun[nq][e], mx);               // finite from below: the running maximum starts at -1e30
-          const float cr = ex2(mrun[nq][e] - mn);
+          const float mn = fmaxf(mrun[nq][e], top(mx));          // finite from below: the running maximum starts at -1e30
+          cr[e] = ex2(mrun[nq][e] - mn);
           mrun[nq][e] = mn;
-          float ls = 0.f, zs = 0.f, wm = 0.f;
-#pragma unroll
-          for (int k = 0; k < U / 16; k++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              float& x = sc[nq][k][2 * h + e];
-              const float p = ex2(x - mn);
-              float w = p * vs[k][h], pz = p * vz[k][h];
-              if (edge && x == -INFINITY) w = pz = 0.f;          // an unseen row may be NaN
-              ls += p;
-              zs += pz;
-              wm = fmaxf(wm, w);
-              x = w;
-            }
-          wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, 4));
-          wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, 8));
-          wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, 16));
-          lrun[nq][e] = fmaf(lrun[nq][e], cr, ls);
-          zrun[nq][e] = fmaf(zrun[nq][e], cr, zs);
-          wrun[nq][e] = fmaxf(wrun[nq][e] * cr, wm);
-          const uint32_t en = min(max(__float_as_uint(wrun[nq][e]) >> 23, 1u), 253u);
-          const int up = min(max((int)erun[nq][e] - (int)en, -126), 126);
-          corr[nq][e] = cr * __uint_as_float((uint32_t)(127 + up) << 23);
-          moved = moved || cr != 1.f || en != erun[nq][e];
-          erun[nq][e] = en;
-          const float vf = __uint_as_float((254u - en) << 23);
-#pragma unroll
-          for (int k = 0; k < U / 16; k++) { sc[nq][k][e] *= vf; sc[nq][k][2 + e] *= vf; }
+          lrun[nq][e] *= cr[e]; zrun[nq][e] *= cr[e]; wtop[nq][e] *= cr[e];
         }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int nq = 0; nq < NQ; nq++)
-#pragma unroll
-          for (int j = 0; j < MT; j++) { o[nq][j][0] *= corr[nq][0]; o[nq][j][1] *= corr[nq][1]; o[nq][j][2] *= corr[nq][0]; o[nq][j][3] *= corr[nq][1]; }
-      }
-#pragma unroll
-      for (int k = 0; k < U / 16; k++) {
-        uint32_t pb[NQ][2];
-#pragma unroll
-        for (int nq = 0; nq < NQ; nq++)
-#pragma unroll
-          for (int h = 0; h < 2; h++) pb[nq][h] = movmatrix_trans(cvt_f16x2(sc[nq][k][2 * h], sc[nq][k][2 * h + 1]));
-        const uint32_t vb = base + k * C::BLOCK + C::V;
-        uint32_t x0[HD / 32 + (HD > C::MAIN)], x1[HD / 32 + (HD > C::MAIN)];      // words of pairs t and t + 4
-        if constexpr (HD == 128) {
-          const uint4 x = lds128(vb + t * 128 + ((g ^ (2 * t)) << 4)), y = lds128(vb + (t + 4) * 128 + ((g ^ (2 * t)) << 4));
-          x0[0] = x.x; x0[1] = x.y; x0[2] = x.z; x0[3] = x.w;
-          x1[0] = y.x; x1[1] = y.y; x1[2] = y.z; x1[3] = y.w;
-        } else {
-          const uint32_t off = (uint32_t)((g * 8) ^ ((t >> 1) * 32));
-          const uint2 x = lds64(vb + t * 64 + off), y = lds64(vb + (t + 4) * 64 + off);
-          x0[0] = x.x; x0[1] = x.y;
-          x1[0] = y.x; x1[1] = y.y;
-          if constexpr (HD > C::MAIN) {
-            x0[2] = kv4_lds32(vb + 512 + t * 16 + (g >> 1) * 4) >> (8 * (g & 1));
-            x1[2] = kv4_lds32(vb + 512 + (t + 4) * 16 + (g >> 1) * 4) >> (8 * (g & 1));
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < MT; j++) {
-          const uint32_t a = x0[j >> 1] >> (8 * (j & 1)), c = x1[j >> 1] >> (8 * (j & 1));
-          const uint32_t A[4] = {kv4_lo(a), kv4_hi(a), kv4_lo(c), kv4_hi(c)};
-#pragma unroll
-          for (int nq = 0; nq < NQ; nq++) mma_f16(o[nq][j], A, pb[nq][0], pb[nq][1]);
-        }
+        scale_o(nq, cr[0], cr[1]);
       }
     }
+    bool large = false;
+#pragma unroll
+    for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+#pragma unroll
+        for (int k = 0; k < U / 16; k++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const int i = 2 * h + e;
+            const float p = ex2(sc[nq][k][i] - mrun[nq][e]);
+            const bool out = EDGE && (unseen[nq] >> (4 * k + i) & 1);      // an unseen row may be NaN
+            const float w = out ? 0.f : p * vs[k][h];
+            lrun[nq][e] += p;
+            zrun[nq][e] = fmaf(p, out ? 0.f : vz[k][h], zrun[nq][e]);
+            wtop[nq][e] = fmaxf(wtop[nq][e], w);
+            sc[nq][k][i] = w;
+          }
+        large = large || wtop[nq][e] > wlim[nq][e];
+      }
+    if (__any_sync(0xffffffffu, large) || moved) {
+#pragma unroll
+      for (int nq = 0; nq < NQ; nq++) {
+        float up[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const uint32_t en = min(max(__float_as_uint(top(wtop[nq][e])) >> 23, 15u), 239u);
+          up[e] = __uint_as_float((uint32_t)(127 + min(max((int)erun[nq][e] - (int)en, -126), 126)) << 23);
+          erun[nq][e] = en;
+          vf[nq][e] = __uint_as_float((254u - en) << 23);
+          wlim[nq][e] = __uint_as_float((en + 14u) << 23);
+        }
+        scale_o(nq, up[0], up[1]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < U / 16; k++) {
+      uint32_t pb[NQ][2];
+#pragma unroll
+      for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) pb[nq][h] = movmatrix_trans(cvt_f16x2(sc[nq][k][2 * h] * vf[nq][0], sc[nq][k][2 * h + 1] * vf[nq][1]));
+      const uint8_t* vb = base + k * C::BLOCK + C::V;
+      uint32_t x0[NW], x1[NW];                                   // words of pairs t and t + 4
+      if constexpr (HD == 128) {
+        const uint4 x = *reinterpret_cast<const uint4*>(vb + t * 128 + ((g ^ (2 * t)) << 4)),
+                    y = *reinterpret_cast<const uint4*>(vb + (t + 4) * 128 + ((g ^ (2 * t)) << 4));
+        x0[0] = x.x; x0[1] = x.y; x0[2] = x.z; x0[3] = x.w;
+        x1[0] = y.x; x1[1] = y.y; x1[2] = y.z; x1[3] = y.w;
+      } else {
+        const uint32_t off = (uint32_t)((g * 8) ^ ((t >> 1) * 32));
+        const uint2 x = *reinterpret_cast<const uint2*>(vb + t * 64 + off), y = *reinterpret_cast<const uint2*>(vb + (t + 4) * 64 + off);
+        x0[0] = x.x; x0[1] = x.y;
+        x1[0] = y.x; x1[1] = y.y;
+        if constexpr (HD > C::MAIN) {
+          x0[2] = *reinterpret_cast<const uint32_t*>(vb + 512 + t * 16 + (g >> 1) * 4) >> (8 * (g & 1));
+          x1[2] = *reinterpret_cast<const uint32_t*>(vb + 512 + (t + 4) * 16 + (g >> 1) * 4) >> (8 * (g & 1));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < MT; j++) {
+        const uint32_t a = x0[j >> 1] >> (8 * (j & 1)), c = x1[j >> 1] >> (8 * (j & 1));
+        const uint32_t A[4] = {a & 0x000F000Fu, a & 0x00F000F0u, c & 0x000F000Fu, c & 0x00F000F0u};
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) mma_f16(o[nq][j], A, pb[nq][0], pb[nq][1]);
+      }
+    }
+  };
+  int st = 0;
+  uint32_t lap = 0;
+#pragma unroll 1
+  for (int i = warp; i < n && warp < W; i += W) {
+    const int k = st * W + warp;
+    if (!mbar_try(&full[k], lap)) ok = mbar_wait(&full[k], lap, wc, W_FULL, 30);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) break;
+    if (!s_skip[k]) {
+      const uint8_t* base = sm + k * F::STAGE;
+      const int slot0 = (u_begin + i) * U;
+      if (slot0 + U > seq.cached) unit(base, slot0, std::true_type());
+      else unit(base, slot0, std::false_type());
+    }
     __syncwarp();                                                // every lane has read the stage
-    issue(i + NST, page_next, st);
-    page_next = page_of(i + NST + 1);
+    if (lane == 0) mbar_arrive(&empty[k]);
     if (++st == NST) { st = 0; lap ^= 1u; }
-  }
-  if (!ok && lane == 0) {                                        // after a failure: this warp's copies in flight
-    const int issued = min(mine, done + NST);
-    for (int i = done; i < issued; i++) drain_phase(&bars[i % NST], (uint32_t)(i / NST) & 1u);
   }
 #pragma unroll
   for (int nq = 0; nq < NQ; nq++)
@@ -627,8 +829,12 @@ __global__ void __launch_bounds__(W * 32) kv4_attn_few(const Kv4Attend P) {
         zrun[nq][e] += __shfl_xor_sync(0xffffffffu, zrun[nq][e], s);
       }
   __syncthreads();                                               // every warp has left its ring
+  if (*s_abort && warp == W && lane < W)                         // after a failure: the copies in flight
+    for (int i = max(0, issued - NST); i < issued; i++)
+      if (i * W + lane < n) drain_phase(&full[i % NST * W + lane], (uint32_t)(i / NST) & 1u);
+  __syncthreads();
   float* part = reinterpret_cast<float*>(sm);
-  {
+  if (warp < W) {
 #pragma unroll
     for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
@@ -638,57 +844,67 @@ __global__ void __launch_bounds__(W * 32) kv4_attn_few(const Kv4Attend P) {
 #pragma unroll
         for (int j = 0; j < MT; j++) {
           const int d = 8 * j < C::MAIN / 2 ? C::MAIN / 8 * g + 2 * j : C::MAIN + 2 * g;
-          *reinterpret_cast<float2*>(pr + d) = make_float2(fmaf(o[nq][j][e], back, zrun[nq][e]), fmaf(o[nq][j][2 + e], back, zrun[nq][e]));
+          *reinterpret_cast<float2*>(pr + d) = make_float2(fmaf(o[nq][j][e] * 0x1p24f, back, zrun[nq][e]), fmaf(o[nq][j][2 + e] * 0x1p20f, back, zrun[nq][e]));
         }
         if (g == 0) *reinterpret_cast<float2*>(pr + HD) = make_float2(mrun[nq][e], lrun[nq][e]);
       }
   }
   __syncthreads();
-  if (ns > 1) cluster_wait();
-  auto merge = [&](const float* p0, int n, int stride, float4& acc, float& mm, float& den) {
-    mm = -1e30f;
-    for (int i = 0; i < n; i++) mm = fmaxf(mm, p0[(size_t)i * stride + HD]);
-    den = 0.f;
-    acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < n; i++) {
-      const float2 ml = *reinterpret_cast<const float2*>(p0 + (size_t)i * stride + HD);
-      const float e = ex2(ml.x - mm);
-      const float4 v = lane < HD / 4 ? *reinterpret_cast<const float4*>(p0 + (size_t)i * stride + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-      den = fmaf(ml.y, e, den);
-      acc.x = fmaf(v.x, e, acc.x); acc.y = fmaf(v.y, e, acc.y); acc.z = fmaf(v.z, e, acc.z); acc.w = fmaf(v.w, e, acc.w);
-    }
-  };
-  auto finish = [&](int lr, const float4& acc, float den) {      // normalise and write local row lr; a row that sees nothing is zeros
-    const int r = r0 + lr;
-    if (r >= rows || lane >= HD / 4) return;
-    const float inv = den == 0.f ? 0.f : 1.f / den;
-    *reinterpret_cast<uint2*>(P.out + (size_t)(seq.first + r / R) * P.o_ld + (size_t)(kvh * R + r % R) * HD + lane * 4) =
-        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-  };
-  for (int lr = warp; lr < ROWS; lr += W) {
+  if (CLUSTER) cluster_wait();
+  for (int lr = warp; lr < min(ROWS, rows - r0); lr += W + 1) {
     float4 acc;
     float mm, den;
-    merge(part + (size_t)lr * PW, W, ROWS * PW, acc, mm, den);
-    if (ns == 1) {
-      finish(lr, acc, den);
-    } else {                                                     // to the CTA that finishes the row
+    kv4_merge<HD>(part + (size_t)lr * PW, min(W, max(n, 1)), ROWS * PW, lane, acc, mm, den);
+    if (!CLUSTER && task.parts == 1) {
+      kv4_finish<HD>(P, seq, kvh, r0 + lr, lane, acc, den);
+    } else if (CLUSTER) {                                        // to the CTA that finishes the row
       const uint32_t to = (uint32_t)(lr % ns), slot = (uint32_t)(rank * ((ROWS + ns - 1) / ns) + lr / ns);
       const uint32_t a = cluster_map(smem_u32(sm + F::INBOX) + slot * PW * 4, to);
       if (lane < HD / 4) st_cluster(a + lane * 16, acc);
       if (lane == 0) st_cluster(a + HD * 4, make_float4(mm, den, 0.f, 0.f));
+    } else {
+      float* w = P.work + ((size_t)blockIdx.x * ROWS + lr) * PW;
+      if (lane < HD / 4) *reinterpret_cast<float4*>(w + lane * 4) = acc;
+      if (lane == 0) *reinterpret_cast<float2*>(w + HD) = make_float2(mm, den);
     }
   }
-  if (ns > 1) {
+  if (CLUSTER) {
     cluster_arrive();
     cluster_wait();
     const int own = (ROWS + ns - 1) / ns;
-    for (int i = warp; i < own && i * ns + rank < ROWS; i += W) {
+    for (int i = warp; i < own && i * ns + rank < min(ROWS, rows - r0); i += W + 1) {
       float4 acc;
       float mm, den;
-      merge(reinterpret_cast<const float*>(sm + F::INBOX) + (size_t)i * PW, ns, own * PW, acc, mm, den);
-      finish(i * ns + rank, acc, den);
+      kv4_merge<HD>(reinterpret_cast<const float*>(sm + F::INBOX) + (size_t)i * PW, ns, own * PW, lane, acc, mm, den);
+      kv4_finish<HD>(P, seq, kvh, r0 + i * ns + rank, lane, acc, den);
     }
   }
+}
+
+// The partials of rows whose positions were split. WARPS 8: as many warps share the parts of a row, grid (row groups, nkv, rows of a group): one long
+// sequence, whose positions are in many parts (37 of 32 K positions by one warp: 5 us more). WARPS 1: a warp a row, grid (row groups, nkv): a
+// batch, whose sequences are in few (48 sequences with eight warps a row: 20 us more).
+template <int HD, int ROWS, int U, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? ROWS * 32 : WARPS * 32) kv4_join(const Kv4Attend P) {
+  constexpr int PW = HD + 4;
+  __shared__ __align__(16) float part[WARPS * PW];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lr = WARPS == 1 ? warp : (int)blockIdx.z, w0 = WARPS == 1 ? 0 : warp;
+  pdl_begin(true);
+  Kv4Task<ROWS, U> task;
+  task.kvh = blockIdx.y;
+  if (!task.template find<true>(P, blockIdx.x, lane, false) || task.parts == 1 || task.r0 + lr >= task.rows) return;
+  const long long t0 = task.task_of(P, 0), step = task.task_of(P, 1) - t0;
+  float4 acc;
+  float mm, den;
+  kv4_merge<HD>(P.work + ((size_t)(t0 + w0 * step) * ROWS + lr) * PW, (task.parts - w0 + WARPS - 1) / WARPS, (size_t)step * WARPS * ROWS * PW, lane, acc, mm, den);
+  if (WARPS > 1) {
+    if (lane < HD / 4) *reinterpret_cast<float4*>(part + warp * PW + lane * 4) = acc;
+    if (lane == 0) *reinterpret_cast<float2*>(part + warp * PW + HD) = make_float2(mm, den);
+    __syncthreads();
+    if (warp) return;
+    kv4_merge<HD>(part, min(WARPS, task.parts), PW, lane, acc, mm, den);
+  }
+  kv4_finish<HD>(P, task.seq, task.kvh, task.r0 + lr, lane, acc, den);
 }
 
 }  // namespace fb

@@ -15,9 +15,10 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _lib
-from .engine import _ptr, _stream_ptr
+from .engine import _ptr, _raw_stream
 
 PAGE = 64                                                  # positions of a page
+NO_SCRATCH = 1344                                          # positions of one sequence up to which attention needs no scratch
 Lengths = Union[int, torch.Tensor]
 
 
@@ -60,10 +61,15 @@ class KvCache4:
         self.pool, self.table = pool, table
         self.layer_bytes = self.n_pages * self.n_kv * record
         self.freq = rope_turns(self.head_dim, float(rope_base), self.device) if rope_base is not None else None
+        self._freq_ptr = _ptr(self.freq)
         self._status = torch.zeros(8, dtype=torch.int32, device=self.device)
         self._index = self.device.index if self.device.index is not None else torch.cuda.current_device()
         self._ld = table.stride(0) if table.shape[0] > 1 else table.shape[1]
-        self._base, self._table_ptr, self._status_ptr = pool.data_ptr(), table.data_ptr(), self._status.data_ptr()
+        self._n_seq = table.shape[0]
+        self._f32 = torch.empty(0, dtype=torch.float32, device=self.device)
+        # what every call says about the cache; a call copies it and adds its own (a call costs the host microseconds, as much as a short kernel)
+        self._proto = bytes(_lib.Kv4Seqs(pool.data_ptr(), table.data_ptr(), None, None, self._status.data_ptr(), 0, self.n_pages, self.n_kv, self.head_dim,
+                                         self._n_seq, self._ld, 0, self._index))
 
     # ------------------------------------------------------------------ plumbing
     @property
@@ -85,48 +91,54 @@ class KvCache4:
             raise _lib.FlintError(st["code"], f"device status {st}")
 
     def _ints(self, t: torch.Tensor, n: int, what: str) -> int:
-        if t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous() or t.numel() != n:
+        if t.dtype is not torch.int32 or t.get_device() != self._index or not t.is_contiguous() or t.numel() != n:
             raise ValueError(f"{what} must be contiguous int32 [{n}] on {self.device}")
         return t.data_ptr()
 
     def _seqs(self, layer: int, n: int, cached: Lengths, start: Optional[torch.Tensor]) -> _lib.Kv4Seqs:
         if not 0 <= layer < self.n_layer:
             raise ValueError(f"layer {layer} of {self.n_layer}")
-        n_seq = self.table.shape[0]
-        if start is None:
-            if n_seq > 1:
-                raise ValueError(f"{n_seq} sequences: `start` says which tokens are whose")
-            start_ptr = None
-        else:
-            start_ptr = self._ints(start, n_seq + 1, "start")
+        s = _lib.Kv4Seqs.from_buffer_copy(self._proto)
+        if layer:
+            s.d_pool += layer * self.layer_bytes
+        s.n_tokens = n
+        if start is not None:
+            s.d_start = self._ints(start, self._n_seq + 1, "start")
+        elif self._n_seq > 1:
+            raise ValueError(f"{self._n_seq} sequences: `start` says which tokens are whose")
         if isinstance(cached, torch.Tensor):
-            cached_ptr, host = self._ints(cached, n_seq, "cached"), 0
+            s.d_cached = self._ints(cached, self._n_seq, "cached")
         else:
-            cached_ptr, host = None, int(cached)
-            if host < 0 or host + (n if start is None else 0) > self.slots:
-                raise ValueError(f"{n} tokens behind {host}: a sequence has {self.slots} slots")
-        return _lib.Kv4Seqs(self._base + layer * self.layer_bytes, self._table_ptr, start_ptr, cached_ptr, self._status_ptr, host, self.n_pages, self.n_kv,
-                            self.head_dim, n_seq, self._ld, n, self._index)
+            if cached < 0 or cached + (n if start is None else 0) > self.slots:
+                raise ValueError(f"{n} tokens behind {cached}: a sequence has {self.slots} slots")
+            s.cached = cached
+        return s
 
-    def _rows(self, t: torch.Tensor, heads: Optional[int], what: str) -> Tuple[torch.Tensor, int]:
-        """bf16 [T, heads, head_dim] as the kernels take it: heads adjacent, tokens a multiple of 16 bytes apart (a copy where it is not so)."""
-        if t.dtype != torch.bfloat16 or t.device != self.device or t.dim() != 3 or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
+    def _rows(self, t: torch.Tensor, heads: Optional[int], what: str) -> Tuple[torch.Tensor, int, int, int]:
+        """(t, its address, T, elements from token to token) of bf16 [T, heads, head_dim] as the kernels take it: heads adjacent, tokens a multiple of 16
+        bytes apart (a copy where it is not so)."""
+        shape = t.shape
+        if t.dtype is not torch.bfloat16 or t.get_device() != self._index or len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
             raise ValueError(f"{what} must be bf16 [T, {heads or 'heads'}, {self.head_dim}] on {self.device}")
-        ld = t.stride(0)
-        if t.shape[0] <= 1:
-            ld = t.shape[1] * self.head_dim
-        if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != self.head_dim) or ld % 8 or ld < t.shape[1] * self.head_dim or t.data_ptr() % 16:
+        T, width, at = shape[0], shape[1] * self.head_dim, t.data_ptr()
+        if t.is_contiguous() and not at & 15:
+            return t, at, T, width
+        ld, to_head, to_dim = t.stride()
+        if T == 1:
+            ld = width
+        if to_dim != 1 or (shape[1] > 1 and to_head != self.head_dim) or ld % 8 or ld < width or at & 15:
             t = t.clone(memory_format=torch.contiguous_format)
-            ld = t.shape[1] * self.head_dim
-        return t, ld
+            return t, t.data_ptr(), T, width
+        return t, at, T, ld
 
-    def _out(self, out: Optional[torch.Tensor], like: torch.Tensor, what: str) -> Tuple[torch.Tensor, int]:
+    def _out(self, out: Optional[torch.Tensor], like: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int]:
         if out is None:
-            return torch.empty(like.shape, dtype=torch.bfloat16, device=self.device), like.shape[1] * self.head_dim
-        got, ld = self._rows(out, like.shape[1], what)
+            out = torch.empty_like(like)                     # contiguous: its heads are adjacent
+            return out, out.data_ptr(), like.shape[1] * self.head_dim
+        got, at, _, ld = self._rows(out, like.shape[1], what)
         if got is not out or out.shape != like.shape:
             raise ValueError(f"{what} must be bf16 {tuple(like.shape)} with adjacent heads, tokens a multiple of 16 bytes apart")
-        return out, ld
+        return out, at, ld
 
     # ------------------------------------------------------------------ launches (asynchronous on the current stream)
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, cached: Lengths, q: Optional[torch.Tensor] = None, start: Optional[torch.Tensor] = None,
@@ -135,21 +147,23 @@ class KvCache4:
         its position on the way; returns q [T, heads, head_dim] rotated (in `q_out` if given, which may be q itself). start int32 [n_seq + 1]: tokens
         start[b] .. start[b+1] - 1 are sequence b's (needed with several sequences). depth int32 [T]: rotation position behind the cached ones, as for a
         tree's nodes; None: the token's place."""
-        k, k_ld = self._rows(k, self.n_kv, "k")
-        v, v_ld = self._rows(v, self.n_kv, "v")
-        T = k.shape[0]
-        if v.shape[0] != T or (q is not None and q.shape[0] != T):
+        k, k_at, T, k_ld = self._rows(k, self.n_kv, "k")
+        v, v_at, Tv, v_ld = self._rows(v, self.n_kv, "v")
+        heads, q_at, q_ld, o_at, o_ld = 0, None, 0, None, 0
+        if q is not None:
+            q, q_at, Tq, q_ld = self._rows(q, None, "q")
+            heads = q.shape[1]
+            q_out, o_at, o_ld = self._out(q_out, q, "q_out")
+        else:
+            Tq, q_out = T, None
+        if T != Tv or T != Tq:
             raise ValueError("q, k and v must have as many tokens")
         s = self._seqs(layer, T, cached, start)
         depth_ptr = None if depth is None else self._ints(depth, T, "depth")
-        heads = q_ld = o_ld = 0
-        if q is not None:
-            q, q_ld = self._rows(q, None, "q")
-            heads = q.shape[1]
-            q_out, o_ld = self._out(q_out, q, "q_out")
-        _lib.check(self.lib.fb_kv4_append(ctypes.byref(s), _ptr(q), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, heads, depth_ptr, _ptr(self.freq),
-                                          _ptr(q_out) if q is not None else None, o_ld, _stream_ptr(self.device)), "fb_kv4_append")
-        return q_out if q is not None else None
+        code = self.lib.fb_kv4_append(ctypes.byref(s), q_at, q_ld, k_at, k_ld, v_at, v_ld, heads, depth_ptr, self._freq_ptr, o_at, o_ld, _raw_stream(self._index))
+        if code:
+            _lib.check(code, "fb_kv4_append")
+        return q_out
 
     def attend(self, layer: int, q: torch.Tensor, cached: Lengths, start: Optional[torch.Tensor] = None, amask: Optional[torch.Tensor] = None,
                scale: Optional[float] = None, max_new: Optional[int] = None, max_len: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -157,47 +171,56 @@ class KvCache4:
         tokens of their own sequence: causal, or those with amask[m, j] != 0 (uint8 or bool [T, new tokens of a sequence], j counted from the sequence's first
         new token). max_new: no sequence has more new tokens (default: T); max_len: about the longest sequence, for cutting the work (default: what `cached`
         says, or all slots). A token that sees nothing gets zeros."""
-        q, q_ld = self._rows(q, None, "q")
-        T, heads = q.shape[0], q.shape[1]
+        q, q_at, T, q_ld = self._rows(q, None, "q")
+        heads = q.shape[1]
         if heads == 0 or heads % self.n_kv:
             raise ValueError(f"{heads} query heads do not share {self.n_kv} kv heads evenly")
         s = self._seqs(layer, T, cached, start)
-        mask_ld = 0
+        mask_at, mask_ld = None, 0
         if amask is not None:
-            if amask.dtype not in (torch.uint8, torch.bool) or amask.device != self.device or amask.dim() != 2 or amask.shape[0] != T or amask.shape[1] < 1:
+            if amask.dtype not in (torch.uint8, torch.bool) or amask.get_device() != self._index or amask.dim() != 2 or amask.shape[0] != T or amask.shape[1] < 1:
                 raise ValueError(f"amask must be uint8 or bool [{T}, new tokens of a sequence] on {self.device}")
             amask = amask.contiguous()
-            mask_ld = amask.shape[1]
+            mask_at, mask_ld = amask.data_ptr(), amask.shape[1]
             if start is None and mask_ld < T:
                 raise ValueError(f"amask must have a column for each of the {T} new tokens")
-        out, o_ld = self._out(out, q, "out")
+        out, o_at, o_ld = self._out(out, q, "out")
         if max_new is None:
             max_new = T
         if max_len is None:
-            max_len = self.slots if isinstance(cached, torch.Tensor) else min(self.slots, int(cached) + max_new)
+            max_len = self.slots if s.d_cached else min(self.slots, cached + max_new)
         if T and (max_new < 1 or max_len < 1):
             raise ValueError("max_new and max_len are at least 1")
-        _lib.check(self.lib.fb_kv4_attend(ctypes.byref(s), q.data_ptr(), q_ld, heads, int(max_new), int(max_len), _ptr(amask), mask_ld,
-                                          self.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(), o_ld, _stream_ptr(self.device)), "fb_kv4_attend")
+        work_at, need, seqs = None, 0, ctypes.byref(s)
+        if self._n_seq > 1 or max_len > NO_SCRATCH:
+            need = self.lib.fb_kv4_attend_bytes(seqs, heads, max_new, max_len)
+            if need:                                         # of the stream's own memory: calls on other streams and other captures have theirs
+                work = torch.empty(need, dtype=torch.uint8, device=self.device)
+                work_at = work.data_ptr()
+        code = self.lib.fb_kv4_attend(seqs, q_at, q_ld, heads, max_new, max_len, mask_at, mask_ld, self.head_dim ** -0.5 if scale is None else scale, o_at, o_ld,
+                                      work_at, need, _raw_stream(self._index))
+        if code:
+            _lib.check(code, "fb_kv4_attend")
         return out
 
     def read(self, layer: Optional[int], n: int, cached: Lengths, start: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """What n rows behind `cached` stand for (the tokens of an append with the same arguments; cached = 0: a sequence's first n): K and V, f32
-        [n, n_kv, head_dim], or with layer None [n_layer, n, n_kv, head_dim]."""
-        s = self._seqs(layer or 0, int(n), cached, start)
-        shape = (n, self.n_kv, self.head_dim) if layer is not None else (self.n_layer, n, self.n_kv, self.head_dim)
-        # rows of tokens that no sequence has are left alone by the kernel
-        new = torch.empty if start is None else torch.zeros
-        k, v = new(shape, dtype=torch.float32, device=self.device), new(shape, dtype=torch.float32, device=self.device)
-        _lib.check(self.lib.fb_kv4_read(ctypes.byref(s), 1 if layer is not None else self.n_layer, self.layer_bytes, k.data_ptr(), v.data_ptr(),
-                                        _stream_ptr(self.device)), "fb_kv4_read")
+        [n, n_kv, head_dim], or with layer None [n_layer, n, n_kv, head_dim]. Tokens that no sequence has: zeros."""
+        s = self._seqs(layer or 0, n, cached, start)
+        shape = (2, n, self.n_kv, self.head_dim) if layer is not None else (2, self.n_layer, n, self.n_kv, self.head_dim)
+        k, v = self._f32.new_empty(shape).unbind(0)
+        code = self.lib.fb_kv4_read(ctypes.byref(s), 1 if layer is not None else self.n_layer, self.layer_bytes, k.data_ptr(), v.data_ptr(), _raw_stream(self._index))
+        if code:
+            _lib.check(code, "fb_kv4_read")
         return k, v
 
     def _one(self, seq: int, cached: int) -> _lib.Kv4Seqs:
-        if not 0 <= seq < self.table.shape[0]:
-            raise ValueError(f"sequence {seq} of {self.table.shape[0]}")
-        return _lib.Kv4Seqs(self._base, self._table_ptr + 4 * seq * self._ld, None, None, self._status_ptr, int(cached), self.n_pages, self.n_kv, self.head_dim, 1,
-                            self._ld if seq < self.table.shape[0] - 1 else self.table.shape[1], 0, self._index)
+        if not 0 <= seq < self._n_seq:
+            raise ValueError(f"sequence {seq} of {self._n_seq}")
+        s = _lib.Kv4Seqs.from_buffer_copy(self._proto)
+        s.d_table += 4 * seq * self._ld
+        s.n_seq, s.cached, s.table_ld = 1, cached, self.table.shape[1]
+        return s
 
     def compact(self, accept: torch.Tensor, pos: int, seq: int = 0):
         """Moves the accepted path's rows of sequence `seq` to slots pos + 1 .. in every layer, from `DecodeEngine.accept_tree`'s output (int32 [2 + nodes] on the
@@ -206,7 +229,7 @@ class KvCache4:
             raise ValueError("accept must be int32 [2 + nodes]")
         s = self._one(seq, pos)
         _lib.check(self.lib.fb_kv4_compact(ctypes.byref(s), self.n_layer, self.layer_bytes, self._ints(accept, accept.numel(), "accept"), accept.numel() - 2,
-                                           _stream_ptr(self.device)), "fb_kv4_compact")
+                                           _raw_stream(self._index)), "fb_kv4_compact")
 
     def move(self, src, dst, seq: int = 0):
         """Slot dst[i] of sequence `seq` takes slot src[i], in order, in every layer."""
@@ -216,4 +239,4 @@ class KvCache4:
         a = (ctypes.c_int32 * n)(*[int(x) for x in src])
         b = (ctypes.c_int32 * n)(*[int(x) for x in dst])
         s = self._one(seq, 0)
-        _lib.check(self.lib.fb_kv4_move(ctypes.byref(s), self.n_layer, self.layer_bytes, a, b, n, _stream_ptr(self.device)), "fb_kv4_move")
+        _lib.check(self.lib.fb_kv4_move(ctypes.byref(s), self.n_layer, self.layer_bytes, a, b, n, _raw_stream(self._index)), "fb_kv4_move")

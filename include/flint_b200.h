@@ -247,9 +247,12 @@ int fb_gemv_static(const void* d_q, const void* d_s, const void* d_z, int32_t ro
  *                   (multiples of 8, 16-byte aligned). d_freq: device uint64 [head_dim / 2], turns per position in units of 2^-64 (half-split pairs), or NULL: no
  *                   rotation. d_depth: rotation position of a token behind its sequence's cached ones (tree nodes), or NULL: its place. d_q may be NULL
  *   fb_kv4_attend : d_out = softmax(scale * q K^T) V over the cached positions and the sequence's own new tokens, which have been appended: causal, or new token j
- *                   where d_amask[m * mask_ld + j] != 0 (m: token of the call). A token that sees nothing gets zeros. max_new: no sequence has more new
- *                   tokens (more: FB_ERR_RANGE in d_status); max_len: about the longest sequence, which decides how the work is cut, not what comes out
- *   fb_kv4_read   : f32 [n_layer][n_tokens][n_kv_head][head_dim], the numbers that the new tokens' rows stand for, bit for bit. d_k or d_v may be NULL
+ *                   where d_amask[m * mask_ld + j] != 0 (m: token of the call). A token that sees nothing gets zeros. max_new and max_len: about the
+ *                   most new tokens and positions of a sequence; they decide how the work is cut, not what comes out.
+ *                   d_work: scratch of fb_kv4_attend_bytes(the same seqs, n_head, max_new, max_len) bytes (0 for one sequence of up to 1344 positions), 16-byte aligned, this call's alone
+ *                   until it has run
+ *   fb_kv4_read   : f32 [n_layer][n_tokens][n_kv_head][head_dim], the numbers that the new tokens' rows stand for, bit for bit (tokens that
+ *                   no sequence has, or whose page is none: zeros). d_k or d_v may be NULL
  *   fb_kv4_compact: fb_kv_compact on sequence 0: slot cached + i takes slot cached + path[i], i = 1 .. len-1, in order; most: entries of the path in d_accept
  *   fb_kv4_move   : fb_kv_move on sequence 0; src / dst are HOST arrays */
 typedef struct fb_kv4_seqs {
@@ -262,7 +265,9 @@ size_t fb_kv4_page_bytes(int32_t n_kv_head, int32_t head_dim);
 int fb_kv4_append(const fb_kv4_seqs* seqs, const void* d_q, int64_t q_ld, const void* d_k, int64_t k_ld, const void* d_v, int64_t v_ld,
                   int32_t n_head, const int32_t* d_depth, const uint64_t* d_freq, void* d_q_out, int64_t qo_ld, void* stream);
 int fb_kv4_attend(const fb_kv4_seqs* seqs, const void* d_q, int64_t q_ld, int32_t n_head, int32_t max_new, int32_t max_len,
-                  const uint8_t* d_amask, int32_t mask_ld, float scale, void* d_out, int64_t o_ld, void* stream);
+                  const uint8_t* d_amask, int32_t mask_ld, float scale, void* d_out, int64_t o_ld, void* d_work, size_t work_bytes,
+                  void* stream);
+size_t fb_kv4_attend_bytes(const fb_kv4_seqs* seqs, int32_t n_head, int32_t max_new, int32_t max_len);
 int fb_kv4_read(const fb_kv4_seqs* seqs, int32_t n_layer, int64_t layer_bytes, float* d_k, float* d_v, void* stream);
 int fb_kv4_compact(const fb_kv4_seqs* seqs, int32_t n_layer, int64_t layer_bytes, const int32_t* d_accept, int32_t most, void* stream);
 int fb_kv4_move(const fb_kv4_seqs* seqs, int32_t n_layer, int64_t layer_bytes, const int32_t* src, const int32_t* dst, int32_t n, void* stream);

@@ -1,11 +1,12 @@
 """GPU: the paged 4-bit K/V cache (append, attention, read-back, moves) against its definition in 64 bits."""
+import ctypes
 import math
 
 import pytest
 import torch
 
 from flint_b200 import _lib
-from flint_b200.kv4 import KvCache4, page_bytes
+from flint_b200.kv4 import NO_SCRATCH, KvCache4, page_bytes
 from tests import kv4_reference as ref
 
 pytestmark = pytest.mark.gpu
@@ -456,12 +457,20 @@ def test_pages_lengths_and_paths_that_cannot_be_are_reported_and_left_out():
         c.append(0, rows(1, 2, nkv, hd), rows(2, 2, nkv, hd), cached, start=begin)
         reported(23)
         c.pool.copy_(pool)
-    c.attend(0, q, ints(100, 60), start=ints(0, 0, 2), max_new=1)                # two new tokens where one was promised
-    reported(23, 1)
     for accept in (ints(5, 0, 0, 1, 2), ints(-1, 0, 0), ints(2, 0, 0, 10 ** 6), ints(2, 0, 0, -50)):
         c.compact(accept, 40)
         reported(24)
         assert torch.equal(c.pool, pool)
+
+
+def test_one_short_sequence_needs_no_scratch():
+    lib, c = _lib.load(), make([64], 2, 64)
+    for nkv in (1, 2, 8, 20, 74, 140):
+        for tokens in (1, 2, 3, 16, 64, 200, 5000):
+            s = c._seqs(0, 0, 0, None)
+            s.n_kv_head, s.n_tokens = nkv, tokens
+            for r in (1, 4, 5, 16):
+                assert lib.fb_kv4_attend_bytes(ctypes.byref(s), nkv * r, tokens, NO_SCRATCH) == 0
 
 
 def test_refused_calls():

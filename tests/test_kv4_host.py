@@ -54,7 +54,7 @@ def test_sequences_that_cannot_be(kw, code):
     s = _seqs(**kw)
     p = ctypes.byref(s)
     assert lib.fb_kv4_append(p, None, 0, 4096, 128, 4096, 128, 4, None, None, None, 0, None) == code
-    assert lib.fb_kv4_attend(p, 4096, 256, 4, 1, 1, None, 0, 1.0, 4096, 256, None) == code
+    assert lib.fb_kv4_attend(p, 4096, 256, 4, 1, 1, None, 0, 1.0, 4096, 256, None, 0, None) == code
     assert lib.fb_kv4_read(p, 1, 0, 4096, 4096, None) == code
 
 
@@ -68,12 +68,12 @@ def test_rows_that_cannot_be():
                dict(depth=4097)):
         assert append(**kw) == A, kw
     attend = lambda q=4096, q_ld=256, nh=4, most=1, length=1, mask=None, m_ld=0, o=4096, o_ld=256: lib.fb_kv4_attend(  # noqa: E731
-        p, q, q_ld, nh, most, length, mask, m_ld, 1.0, o, o_ld, None)
+        p, q, q_ld, nh, most, length, mask, m_ld, 1.0, o, o_ld, None, 0, None)
     for kw in (dict(q=None), dict(o=None), dict(q=4100), dict(q_ld=255), dict(o_ld=8), dict(most=0), dict(length=0), dict(mask=4096, m_ld=0)):
         assert attend(**kw) == A, kw
     assert attend(nh=3) == _lib.FB_ERR_SHAPE and attend(nh=0) == _lib.FB_ERR_SHAPE
     several = _seqs(n_seq=2)
-    assert lib.fb_kv4_attend(ctypes.byref(several), 4096, 256, 4, 1, 1, None, 0, 1.0, 4096, 256, None) == A      # whose tokens?
+    assert lib.fb_kv4_attend(ctypes.byref(several), 4096, 256, 4, 1, 1, None, 0, 1.0, 4096, 256, None, 0, None) == A      # whose tokens?
     for n_layer, layer in ((0, 0), (70000, 0), (1, 8), (1, -16)):
         assert lib.fb_kv4_read(p, n_layer, layer, 4096, 4096, None) == A
         assert lib.fb_kv4_compact(p, n_layer, layer, 4096, 1, None) == A
