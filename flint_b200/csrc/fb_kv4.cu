@@ -3,10 +3,13 @@
 #include <string.h>
 #include <stdlib.h>
 #include <stdio.h>
+#include <stdlib.h>
+#include <stdio.h>
 
 #include "../../include/flint_b200.h"
 #include "fb_ctx.hpp"
 #include "fb_kv4.cuh"
+#include "fb_kv4_tc.cuh"
 
 using namespace fb;
 
@@ -55,9 +58,16 @@ int done(cudaError_t e) { return e == cudaSuccess ? FB_OK : FB_ERR_CUDA; }
 struct Kv4Geometry { int rows; int64_t groups, ctas; int nsplit, slots, chunk; };
 Kv4Geometry few_geometry(int n_seq, int n_tokens, int nkv, int r, int max_new, int max_len, int sms) {
   Kv4Geometry g{(int64_t)max_new * r <= 8 ? 8 : 16, 0, 0, 1, 0, 8};
+  int from = 65, slots = -1, chunk = 2;
+  if (getenv("KV4")) sscanf(getenv("KV4"), "%d,%d,%d", &from, &slots, &chunk);
+  if ((int64_t)max_new * r >= from) g.rows = kManyRows;
   g.groups = n_seq == 1 ? ((int64_t)n_tokens * r + g.rows - 1) / g.rows : (int64_t)n_tokens * r / g.rows + n_seq;
   const int64_t units = ((int64_t)max_len + 31) / 32, items = g.groups * nkv;
-  if (n_seq == 1) {
+  if (g.rows == kManyRows) {
+    g.chunk = chunk;
+    if (items * 3 < sms * 2) g.slots = sms;
+    if (slots >= 0) g.slots = slots;
+  } else if (n_seq == 1) {
     while (g.nsplit < 8 && items * g.nsplit * 2 <= (g.nsplit == 4 ? sms * 2 / 3 : sms) && units >= g.nsplit * 2 * 4) g.nsplit *= 2;
     if (units > (int64_t)6 * kFewWarps * g.nsplit && items * g.nsplit <= sms) { g.nsplit = 1; g.slots = 2 * sms; }
   } else if (units > 12 * kFewWarps && items <= 8 * (int64_t)sms) {
@@ -97,7 +107,22 @@ cudaError_t launch_few(Kv4Attend p, const Kv4Geometry& g, cudaStream_t st) {
   if (e != cudaSuccess || !g.slots) return e;
   if (p.S.n_seq == 1)
     return launch_pdl(kv4_join<HD, F::ROWS, F::U, 8>, dim3((unsigned)g.groups, (unsigned)p.S.nkv, F::ROWS), dim3(256), 0, st, p);
-  return launch_pdl(kv4_join<HD, F::ROWS, F::U, 1>, dim3((unsigned)g.groups, (unsigned)p.S.nkv), dim3(F::ROWS * 32), 0, st, p);
+  return launch_pdl(kv4_join<HD, F::ROWS, F::U, 1>, dim3((unsigned)g.groups, (unsigned)p.S.nkv, F::ROWS / 8), dim3(256), 0, st, p);
+}
+template <int HD>
+cudaError_t launch_many(Kv4Attend p, const Kv4Geometry& g, cudaStream_t st) {
+  static bool done[64] = {};
+  p.nsplit = 1; p.slots = g.slots; p.chunk = g.chunk;
+  if (g.groups > 0x7fffffff || g.ctas > 0x7fffffff) return cudaErrorInvalidValue;
+  cudaError_t e = configure_few(kv4_attn_many<HD>, Kv4Many<HD>::TOTAL, done);
+  if (e == cudaSuccess) e = launch_pdl(kv4_attn_many<HD>, dim3((unsigned)g.ctas), dim3(kManyThreads), (size_t)Kv4Many<HD>::TOTAL, st, p);
+  if (e == cudaSuccess && g.slots)
+    e = launch_pdl(kv4_join<HD, kManyRows, kManyStep, 1>, dim3((unsigned)g.groups, (unsigned)p.S.nkv, kManyRows / 8), dim3(256), 0, st, p);
+  return e;
+}
+template <int HD>
+cudaError_t launch_attend(const Kv4Attend& p, const Kv4Geometry& g, cudaStream_t st) {
+  return g.rows == kManyRows ? launch_many<HD>(p, g, st) : (g.rows == 8 ? launch_few<HD, 1, kFewWarps>(p, g, st) : launch_few<HD, 2, kFewWarps>(p, g, st));
 }
 
 }  // namespace
@@ -222,16 +247,15 @@ int kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n_he
   const Kv4Geometry geo = few_geometry(s->n_seq, s->n_tokens, s->n_kv_head, p.R, max_new < s->n_tokens ? max_new : s->n_tokens, max_len, sms);
   if (few_work(geo, s->head_dim) > work_bytes || ((uintptr_t)work & 15)) return FB_ERR_ARG;
   p.work = work;
-  const bool one = geo.rows == 8;
   switch (s->head_dim) {
-    case 64: return done(one ? launch_few<64, 1, kFewWarps>(p, geo, st) : launch_few<64, 2, 7>(p, geo, st));
-    case 80: return done(one ? launch_few<80, 1, kFewWarps>(p, geo, st) : launch_few<80, 2, 7>(p, geo, st));
-    default: return done(one ? launch_few<128, 1, kFewWarps>(p, geo, st) : launch_few<128, 2, 7>(p, geo, st));
+    case 64: return done(launch_attend<64>(p, geo, st));
+    case 80: return done(launch_attend<80>(p, geo, st));
+    default: return done(launch_attend<128>(p, geo, st));
   }
 }
 
 // one sequence is split over clusterless CTAs only while its row groups are fewer than the SMs
-size_t kv4_attend_most(int n_kv_head, int head_dim, int sms) { return (size_t)(3 * sms + n_kv_head) * 16 * (head_dim + 4) * 4; }
+size_t kv4_attend_most(int n_kv_head, int head_dim, int sms) { return (size_t)(2 * sms + n_kv_head) * kManyRows * (head_dim + 4) * 4; }
 
 size_t fb_kv4_attend_bytes(const fb_kv4_seqs* s, int32_t n_head, int32_t max_new, int32_t max_len) {
   if (!s || s->n_kv_head < 1 || s->n_kv_head > 65535 || n_head < 1 || n_head % s->n_kv_head || max_new < 1 || max_len < 1 || s->n_seq < 0) return 0;

@@ -882,13 +882,13 @@ __global__ void __launch_bounds__(W * 32 + 32) kv4_attn_few(const Kv4Attend P) {
 }
 
 // The partials of rows whose positions were split. WARPS 8: as many warps share the parts of a row, grid (row groups, nkv, rows of a group): one long
-// sequence, whose positions are in many parts (37 of 32 K positions by one warp: 5 us more). WARPS 1: a warp a row, grid (row groups, nkv): a
-// batch, whose sequences are in few (48 sequences with eight warps a row: 20 us more).
+// sequence, whose positions are in many parts (37 of 32 K positions by one warp: 5 us more). WARPS 1: a warp a row, eight rows a CTA, grid (row groups, nkv, rows /
+// 8): a batch, whose sequences are in few (48 sequences with eight warps a row: 20 us more), and the many rows of kv4_attn_many.
 template <int HD, int ROWS, int U, int WARPS>
-__global__ void __launch_bounds__(WARPS == 1 ? ROWS * 32 : WARPS * 32) kv4_join(const Kv4Attend P) {
+__global__ void __launch_bounds__(256) kv4_join(const Kv4Attend P) {
   constexpr int PW = HD + 4;
   __shared__ __align__(16) float part[WARPS * PW];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lr = WARPS == 1 ? warp : (int)blockIdx.z, w0 = WARPS == 1 ? 0 : warp;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lr = WARPS == 1 ? (int)blockIdx.z * 8 + warp : (int)blockIdx.z, w0 = WARPS == 1 ? 0 : warp;
   pdl_begin(true);
   Kv4Task<ROWS, U> task;
   task.kvh = blockIdx.y;

@@ -1,0 +1,400 @@
+// Attention of many query rows over the paged 4-bit cache on the 5th-generation tensor cores (tcgen05): prompts and large trees.
+//
+// A CTA takes 256 query rows (row = token * R + head of the group) of a sequence and kv head as two tiles of 128, and its task's positions in steps of
+// 128 (two pages). Per step and tile: S[128 rows][128 positions] = Q K^T into tensor memory, softmax by a warpgroup (a thread a row: no shuffles), P as bf16 back
+// into tensor memory over S, O[128][HD] += P V. Tensor pipe and exponentials (16 a clock and SM) need the same 1024 clocks a tile and step at heads of 128, so the two
+// tiles take turns: one multiplies while the other exponentiates. Keys and values are dequantised once for both tiles by eight warps into the K-major
+// 128-byte-swizzle layout that the MMA reads, K as [position][dim], V as [dim][position]: (nib - 8) s + z in bf16, rounded once, the precision of a bf16 cache (half
+// a step is 2^-8), and with bf16's range, so that rows of any size stand side by side. (Operands nib - 8, with s and z in the softmax as kv4_attn_few has
+// them, would be exact, but cost the softmax, which is what bounds this kernel, twice its instructions.) P is bf16 as well, sums and maxima are fp32.
+// The maximum is moved, and O rescaled, only when a score exceeds it by more than 2^8.
+// Warps: 0..3 and 4..7 softmax of tiles 0 and 1 (and Q in, O out), 8..15 dequantise, 16 brings pages (one bulk copy each), 17 issues MMAs.
+#pragma once
+#include "fb_kv4.cuh"
+#include "fb_tcgen.cuh"
+
+namespace fb {
+
+constexpr int kManyThreads = 18 * 32, kManyRows = 256, kManyStep = 128;
+
+template <int HD>
+struct Kv4Many {
+  static constexpr int REC = Kv4<HD>::REC, NB = HD == 64 ? 1 : 2;           // blocks of 64 dims of a K-major tile
+  static constexpr int QT = NB * 128 * 128, KT = NB * kManyStep * 128, VT = HD * 128;      // bytes: Q tile, K step, V page
+  static constexpr int NR = 3;                                              // pages in flight
+  static constexpr int Q = 0, K = Q + 2 * QT, V = K + 2 * KT, RAW = V + 4 * VT, BAR = RAW + NR * REC;
+  static constexpr int TOTAL = BAR + 256 + 1024;                            // + slack to align the base
+  static constexpr int T_S = 0, T_O = 256, TCOLS = 512;                     // tensor memory columns: two S / P, two O
+  static_assert(TOTAL <= 227 * 1024 && T_O + 2 * HD <= TCOLS && QT % 1024 == 0 && VT % 1024 == 0 && RAW % 16 == 0 && REC % 16 == 0, "plan");
+};
+
+__device__ __forceinline__ uint32_t kv4_dequant2(uint32_t w, __nv_bfloat162 s, __nv_bfloat162 z) {       // nibbles in bits 0..3 and 16..19
+  const uint32_t x = (w & 0x000F000Fu) | 0x43004300u;            // 128 + nib
+  const uint32_t k136 = 0x43084308u;
+  const __nv_bfloat162 r = __hfma2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&k136)), s, z);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ __nv_bfloat162 kv4_bf2(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
+
+// after a failure: the copies and MMAs in flight
+template <int NR>
+inline __device__ __noinline__ void many_drain(uint64_t* raw_full, uint64_t* s_full, uint64_t* pv_done, volatile int* s_issued) {
+  drain_ring<NR>(raw_full, (uint32_t)s_issued[0]);
+  for (int t = 0; t < 2; t++) {
+    if (s_issued[1 + t]) drain_phase(&s_full[t], (uint32_t)(s_issued[1 + t] - 1) & 1u);
+    if (s_issued[3 + t]) drain_phase(&pv_done[t], (uint32_t)(s_issued[3 + t] - 1) & 1u);
+  }
+  __syncwarp();
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend P) {
+  using C = Kv4<HD>;
+  using M = Kv4Many<HD>;
+  constexpr int NR = M::NR, REC = M::REC, KS = HD / 16;
+  extern __shared__ __align__(1024) uint8_t tsm_raw[];
+  uint8_t* sm = tsm_raw + ((1024u - (smem_u32(tsm_raw) & 1023u)) & 1023u);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + M::BAR);
+  uint64_t *raw_full = bars, *raw_empty = raw_full + NR, *k_full = raw_empty + NR, *k_empty = k_full + 2, *v_full = k_empty + 2, *v_empty = v_full + 2,
+           *s_full = v_empty + 2, *p_full = s_full + 2, *pv_done = p_full + 2, *q_full = pv_done + 2;
+  unsigned long long* s_bad = reinterpret_cast<unsigned long long*>(q_full + 1);       // [2 steps][2 pages] positions whose V is NaN
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_bad + 4);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+  volatile int* s_issued = s_abort + 1;                          // [5] pages, QK of tiles 0 and 1, PV of tiles 0 and 1
+  volatile int* s_none = s_issued + 5;                           // [NR] the page does not exist
+  volatile int* s_gone = s_none + NR;                            // [2 steps] bit p: page p of the step does not exist
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Kv4Seqs& S = P.S;
+  pdl_begin(true);
+  Kv4Task<kManyRows, kManyStep> task;
+  if (!task.template find<false>(P, blockIdx.x, lane, blockIdx.x == 0 && warp == 0) || (task.n <= 0 && task.parts == 1)) return;
+  const Kv4Seq& seq = task.seq;
+  const int rows = task.rows - task.r0, tiles = rows > 128 ? 2 : 1, n = max(task.n, 0), kvh = task.kvh, total = task.total;
+  if (tid == 0) {
+    for (int i = 0; i < NR; i++) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 8); }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&k_full[i], 8); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 8); mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(q_full, 4 * tiles);
+    *s_abort = 0;
+    for (int i = 0; i < 5; i++) s_issued[i] = 0;
+    mbar_fence_init();
+  }
+  if (warp == 17) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(M::TCOLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  const WaitCtl wc{S.status, s_abort, P.spin_limit};
+  bool ok = true;
+
+  if (warp == 16) {
+    // ---------------- pages, two a step; a page behind the last position or that the table does not have is left out
+    int r = 0, issued = 0, page = 0;
+    uint32_t lap = 1;
+    const int pages = 2 * n, p_end = (total + kPage - 1) / kPage;
+    for (; issued < pages && ok; issued++) {
+      if ((issued & 31) == 0) {
+        const int p = 2 * task.unit + issued + lane;
+        page = issued + lane < pages && p < p_end ? kv4_page(S, task.b, p * kPage, true) : -1;
+      }
+      const int now = __shfl_sync(0xffffffffu, page, issued & 31);
+      ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[r], lap, wc, W_EMPTY, 40));
+      if (!ok) break;
+      if (lane == 0) {
+        s_none[r] = now < 0;
+        if (now < 0) {
+          mbar_arrive(&raw_full[r]);
+        } else {
+          mbar_expect_tx(&raw_full[r], REC);
+          bulk_g2s(sm + M::RAW + r * REC, kv4_block<HD>(S, now, kvh, 0), REC, &raw_full[r]);
+        }
+      }
+      if (++r == NR) { r = 0; lap ^= 1u; }
+    }
+    if (lane == 0) s_issued[0] = issued;
+  } else if (warp == 17) {
+    // ---------------- MMA issue: per tile PV of a step, then QK of the next one once PV has read P, which lies over S
+    constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);               // bf16 x bf16 -> fp32, 128 rows
+    auto qk = [&](int t, int i) {
+      const int b = i & 1;
+      if (elect_one()) {
+        const uint64_t qa = tc_desc(smem_u32(sm + M::Q + t * M::QT)), kb = tc_desc(smem_u32(sm + M::K + b * M::KT));
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+          const uint64_t off = (uint64_t)(((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4);
+          tc_mma_ss(tmem + M::T_S + t * 128, qa + off, kb + off, idesc | ((128u >> 3) << 17), k ? 1u : 0u);
+        }
+        tc_commit(&s_full[t]);
+        if (t == tiles - 1) tc_commit(&k_empty[b]);
+      }
+      __syncwarp();
+      if (lane == 0) s_issued[1 + t] = i + 1;
+    };
+    auto pv = [&](int t, int i) {
+      const int b = i & 1;
+      if (elect_one()) {
+        const uint64_t vb = tc_desc(smem_u32(sm + M::V + b * 2 * M::VT));
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          tc_mma_ts(tmem + M::T_O + t * HD, tmem + M::T_S + t * 128 + k * 8, vb + (uint64_t)(((k >> 2) * M::VT + (k & 3) * 32) >> 4),
+                    idesc | ((uint32_t)(HD >> 3) << 17), i || k ? 1u : 0u);
+        tc_commit(&pv_done[t]);
+        if (t == tiles - 1) tc_commit(&v_empty[b]);
+      }
+      __syncwarp();
+      if (lane == 0) s_issued[3 + t] = i + 1;
+    };
+    auto wait = [&](uint64_t* bar, int i, int where) {           // phase i of a barrier
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, (uint32_t)i & 1u, wc, W_FULL, where));
+      tc_fence_after();
+      return ok;
+    };
+    if (n > 0 && wait(q_full, 0, 41) && wait(&k_full[0], 0, 42))
+      for (int t = 0; t < tiles; t++) qk(t, 0);
+    for (int i = 0; i < n && ok; i++)
+      for (int t = 0; t < tiles && ok; t++) {
+        if (!wait(&p_full[t], i, 43) || (t == 0 && !wait(&v_full[i & 1], i >> 1, 44))) break;
+        pv(t, i);
+        if (i + 1 < n) {
+          if ((t == 0 && !wait(&k_full[(i + 1) & 1], (i + 1) >> 1, 45)) || !wait(&pv_done[t], i, 46)) break;
+          qk(t, i + 1);
+        }
+      }
+  } else if (warp >= 8) {
+    // ---------------- dequantise: per page K (tasks of two words: 16 dims of a position), then V (tasks of four words: four dims of eight positions)
+    const int dw = warp - 8;
+    int r = 0;
+    uint32_t lap = 0;
+    for (int i = 0; i < n && ok; i++) {
+      const int b = i & 1;
+      if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[b], (uint32_t)((i >> 1) - 1) & 1u, wc, W_EMPTY, 47) &&
+                                                   mbar_wait(&v_empty[b], (uint32_t)((i >> 1) - 1) & 1u, wc, W_EMPTY, 48));
+      for (int h = 0; h < 2 && ok; h++) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[r], lap, wc, W_FULL, 49));
+        if (!ok) break;
+        const uint8_t* rec = sm + M::RAW + r * REC;
+        uint8_t *kt = sm + M::K + b * M::KT + h * (kPage * 128), *vt = sm + M::V + (2 * b + h) * M::VT;
+        const int left = total - ((task.unit + i) * kManyStep + h * kPage);      // positions of the page that exist
+        const bool none = s_none[r] != 0 || left <= 0;
+        // V's NaN rows, and what lies behind the last position, become zeros here: every row of P multiplies them
+        unsigned long long bad = 0;
+        if (!none) {
+          const uint32_t a = *reinterpret_cast<const uint32_t*>(rec + (lane >> 4) * C::BLOCK + C::VSZ + (lane & 15) * 4),
+                         c = *reinterpret_cast<const uint32_t*>(rec + (2 + (lane >> 4)) * C::BLOCK + C::VSZ + (lane & 15) * 4);
+          bad = (unsigned long long)__ballot_sync(0xffffffffu, lane < left && !(bflo(a) < INFINITY)) |
+                (unsigned long long)__ballot_sync(0xffffffffu, lane + 32 < left && !(bflo(c) < INFINITY)) << 32;
+        }
+        const bool special = bad != 0 || left < kPage;
+        if (dw == 0 && lane == 0) {
+          s_bad[2 * b + h] = bad;
+          if (h == 0) s_gone[b] = none;
+          else if (none) s_gone[b] = s_gone[b] | 2;
+        }
+        if (!none) {
+          auto key = [&](int p, int q) {                         // words 2q, 2q + 1 of position p
+            const uint8_t* blk = rec + (p >> 4) * C::BLOCK;
+            const uint2 w = *reinterpret_cast<const uint2*>(blk + C::k_word(p & 15, 2 * q));
+            const uint32_t sz = *reinterpret_cast<const uint32_t*>(blk + C::KSZ + (p & 15) * 4);
+            const __nv_bfloat162 s = kv4_bf2(__byte_perm(sz, sz, 0x1010)), z = kv4_bf2(__byte_perm(sz, sz, 0x3232));
+            uint8_t* row = kt + (q >> 2) * (kManyStep * 128) + p * 128;
+            const uint32_t x[2] = {w.x, w.y};
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+              *reinterpret_cast<uint4*>(row + ((((2 * q + e) & 7) ^ (p & 7)) << 4)) =
+                  make_uint4(kv4_dequant2(x[e], s, z), kv4_dequant2(x[e] >> 4, s, z), kv4_dequant2(x[e] >> 8, s, z), kv4_dequant2(x[e] >> 12, s, z));
+          };
+          if constexpr (HD == 128) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) key((dw + 8 * e) * 4 + (lane >> 3), lane & 7);
+          } else {
+            key(dw * 8 + (lane >> 2), lane & 3);
+            if (HD == 80 && dw < 2) key(dw * 32 + lane, 4);
+          }
+        }
+        auto value = [&](int c, int w) {                         // dims 4w .. 4w+3 of positions 8c .. 8c+7
+          const uint8_t* blk = rec + (c >> 1) * C::BLOCK;
+          uint32_t out[4][4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const int u = (c & 1) * 4 + k;
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(blk + C::v_word(u, w));
+            uint2 sz = *reinterpret_cast<const uint2*>(blk + C::VSZ + u * 8);
+            if (special) {
+              if (none || 8 * c + 2 * k >= left || !(bflo(sz.x) < INFINITY)) sz.x = 0;
+              if (none || 8 * c + 2 * k + 1 >= left || !(bflo(sz.y) < INFINITY)) sz.y = 0;
+            }
+            const __nv_bfloat162 s = kv4_bf2(__byte_perm(sz.x, sz.y, 0x5410)), z = kv4_bf2(__byte_perm(sz.x, sz.y, 0x7632));
+#pragma unroll
+            for (int e = 0; e < 4; e++) out[e][k] = kv4_dequant2(x >> (4 * e), s, z);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int d = 4 * w + e;
+            *reinterpret_cast<uint4*>(vt + d * 128 + ((c ^ (d & 7)) << 4)) = make_uint4(out[e][0], out[e][1], out[e][2], out[e][3]);
+          }
+        };
+        if (none) {
+          for (int k = tid - 256; k < M::VT / 16; k += 256) *reinterpret_cast<uint4*>(vt + k * 16) = make_uint4(0, 0, 0, 0);
+        } else {
+          // a phase of eight lanes stores to eight chunks; four chunks' lanes read words of different bank groups
+          const int ci = (lane >> 1) & 3, wi = (lane & 1) | (lane >> 3) << 1;
+          constexpr int NG = C::MAIN / 32;                       // groups of eight words
+          if (dw < 2 * NG) value(4 * (dw & 1) + ci, 8 * (((dw >> 1) + ci) & (NG - 1)) + wi);
+          if (HD == 80 && dw == 7) value((lane >> 1) & 7, 16 + ((lane & 1) | (lane >> 4) << 1));
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&raw_empty[r]);
+        if (++r == NR) { r = 0; lap ^= 1u; }
+      }
+      if (!ok) break;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) { mbar_arrive(&k_full[b]); mbar_arrive(&v_full[b]); }
+    }
+  } else if (warp >> 2 < tiles) {
+    // ---------------- softmax of tile t: thread = row
+    const int t = warp >> 2, row = tid & 127, lr = t * 128 + row, R = P.R;
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = tl + M::T_S + t * 128, to = tl + M::T_O + t * HD;
+    const bool live = lr < rows;
+    const int gr = task.r0 + min(lr, rows - 1), mq = gr / R, head = kvh * R + gr % R;
+    {                                                            // Q: the row into the swizzled tile; a negative scale is a negative Q
+      const uint16_t* src = P.q + (size_t)(seq.first + mq) * P.q_ld + (size_t)head * HD;
+      const uint32_t flip = P.scale < 0.f ? 0x80008000u : 0u;
+      uint8_t* qt = sm + M::Q + t * M::QT + row * 128;
+#pragma unroll
+      for (int c = 0; c < HD / 8; c++) {
+        uint4 v = live ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+        v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+        *reinterpret_cast<uint4*>(qt + (c >> 3) * (128 * 128) + (((c & 7) ^ (row & 7)) << 4)) = v;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    const float cs = fmaxf(fabsf(P.scale), 1e-30f);              // not zero: a score that is not seen stays -inf
+    const uint8_t* mask = P.amask ? P.amask + (size_t)(seq.first + mq) * P.mask_ld : nullptr;
+    float m = -1e30f, l = 0.f;
+    for (int i = 0; i < n; i++) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], (uint32_t)i & 1u, wc, W_FULL, 50));
+      if (!ok) break;
+      tc_fence_after();
+      // the step's V is dequantised by now or soon: its flags are needed only where something is special
+      const int p0 = (task.unit + i) * kManyStep, gone = s_gone[i & 1];
+      const bool edge = p0 + kManyStep > seq.cached || gone;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        uint32_t v[32];
+        tc_ld32(ts + c * 32, v);
+        tc_ld_wait();
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 32; e++) {
+            const int tp = p0 + c * 32 + e, j = tp - seq.cached;
+            bool see = tp < total && !(gone >> (c >> 1) & 1);
+            if (see && j >= 0) see = mask ? j < P.mask_ld && mask[j] != 0 : j <= mq;
+            if (!see) v[e] = 0xff800000u;
+          }
+          __syncwarp();
+          tc_st32(ts + c * 32, v);
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e++) mx = fmaxf(mx, __uint_as_float(v[e]));
+      }
+      if (edge) tc_st_wait();
+      const float top = mx * cs;
+      if (__any_sync(0xffffffffu, top > m + 8.f)) {
+        const float mn = fmaxf(m, top), corr = ex2(m - mn);
+        if (i > 0) {                                             // O as the steps before left it
+          ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (uint32_t)(i - 1) & 1u, wc, W_FULL, 51));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 16) {
+            uint32_t v[16];
+            tc_ld16(to + c, v);
+            tc_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * corr);
+            tc_st16(to + c, v);
+          }
+        }
+        m = mn;
+        l *= corr;
+      }
+      const unsigned long long bad0 = s_bad[2 * (i & 1)], bad1 = s_bad[2 * (i & 1) + 1];
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        uint32_t v[32], o[16];
+        tc_ld32(ts + c * 32, v);
+        tc_ld_wait();
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const float a = ex2(fmaf(__uint_as_float(v[2 * e]), cs, -m)), d = ex2(fmaf(__uint_as_float(v[2 * e + 1]), cs, -m));
+          s0 += a;
+          s1 += d;
+          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[e]) : "f"(d), "f"(a));
+        }
+        l += s0 + s1;
+        if (bad0 | bad1) {                                       // a row of V that is NaN, for the rows that see it
+          const uint32_t bad = (uint32_t)((c < 2 ? bad0 : bad1) >> (32 * (c & 1)));
+#pragma unroll
+          for (int e = 0; e < 32; e++)
+            if ((bad >> e & 1) && v[e] != 0xff800000u) l = __uint_as_float(0x7fc00000u);
+        }
+        tc_st16(ts + c * 16, o);
+      }
+      tc_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[t]);
+    }
+    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (uint32_t)(n - 1) & 1u, wc, W_FULL, 52));
+    tc_fence_after();
+    if (ok) {
+      const float inv = task.parts > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+      uint16_t* out = P.out + (size_t)(seq.first + mq) * P.o_ld + (size_t)head * HD;
+      float* w = task.parts > 1 ? P.work + ((size_t)blockIdx.x * kManyRows + lr) * (HD + 4) : nullptr;
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 16) {
+        uint32_t v[16];
+        if (n > 0) {
+          tc_ld16(to + c, v);
+          tc_ld_wait();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; e++) v[e] = 0;
+        }
+        float f[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++) f[e] = l == 0.f ? 0.f : __uint_as_float(v[e]) * inv;
+        if (!live) {
+        } else if (w) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(w + c + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; e += 8)
+            *reinterpret_cast<uint4*>(out + c + e) =
+                make_uint4(pack_bf16(f[e], f[e + 1]), pack_bf16(f[e + 2], f[e + 3]), pack_bf16(f[e + 4], f[e + 5]), pack_bf16(f[e + 6], f[e + 7]));
+        }
+        __syncwarp();
+      }
+      if (w && live) *reinterpret_cast<float2*>(w + HD) = make_float2(m, l);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 17) {
+    if (*s_abort) many_drain<NR>(raw_full, s_full, pv_done, s_issued);
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(M::TCOLS));
+  }
+}
+
+}  // namespace fb

@@ -18,7 +18,7 @@ from . import _lib
 from .engine import _ptr, _raw_stream
 
 PAGE = 64                                                  # positions of a page
-NO_SCRATCH = 1344                                          # positions of one sequence up to which attention needs no scratch
+NO_SCRATCH = (1344, 64)                                    # positions of one sequence, and query rows of a kv head, up to which attention needs no scratch
 Lengths = Union[int, torch.Tensor]
 
 
@@ -192,7 +192,7 @@ class KvCache4:
         if T and (max_new < 1 or max_len < 1):
             raise ValueError("max_new and max_len are at least 1")
         work_at, need, seqs = None, 0, ctypes.byref(s)
-        if self._n_seq > 1 or max_len > NO_SCRATCH:
+        if self._n_seq > 1 or max_len > NO_SCRATCH[0] or max_new * heads > NO_SCRATCH[1] * self.n_kv:
             need = self.lib.fb_kv4_attend_bytes(seqs, heads, max_new, max_len)
             if need:                                         # of the stream's own memory: calls on other streams and other captures have theirs
                 work = torch.empty(need, dtype=torch.uint8, device=self.device)

@@ -249,7 +249,8 @@ int fb_gemv_static(const void* d_q, const void* d_s, const void* d_z, int32_t ro
  *   fb_kv4_attend : d_out = softmax(scale * q K^T) V over the cached positions and the sequence's own new tokens, which have been appended: causal, or new token j
  *                   where d_amask[m * mask_ld + j] != 0 (m: token of the call). A token that sees nothing gets zeros. max_new and max_len: about the
  *                   most new tokens and positions of a sequence; they decide how the work is cut, not what comes out.
- *                   d_work: scratch of fb_kv4_attend_bytes(the same seqs, n_head, max_new, max_len) bytes (0 for one sequence of up to 1344 positions), 16-byte aligned, this call's alone
+ *                   d_work: scratch of fb_kv4_attend_bytes(the same seqs, n_head, max_new, max_len) bytes (0 for one sequence of up to 1344 positions and 64 query rows a
+ *                   kv head), 16-byte aligned, this call's alone
  *                   until it has run
  *   fb_kv4_read   : f32 [n_layer][n_tokens][n_kv_head][head_dim], the numbers that the new tokens' rows stand for, bit for bit (tokens that
  *                   no sequence has, or whose page is none: zeros). d_k or d_v may be NULL
