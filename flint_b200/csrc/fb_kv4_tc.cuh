@@ -8,14 +8,15 @@
 // a step is 2^-8), and with bf16's range, so that rows of any size stand side by side. (Operands nib - 8, with s and z in the softmax as kv4_attn_few has
 // them, would be exact, but cost the softmax, which is what bounds this kernel, twice its instructions.) P is bf16 as well, sums and maxima are fp32.
 // The maximum is moved, and O rescaled, only when a score exceeds it by more than 2^8.
-// Warps: 0..3 and 4..7 softmax of tiles 0 and 1 (and Q in, O out), 8..15 dequantise, 16 brings pages (one bulk copy each), 17 issues MMAs.
+// Warps: 0..3 and 4..7 softmax of tiles 0 and 1 (and Q in, O out), 8..13 dequantise, 14 brings pages (one bulk copy each), 15 issues MMAs.
 #pragma once
 #include "fb_kv4.cuh"
 #include "fb_tcgen.cuh"
 
 namespace fb {
 
-constexpr int kManyThreads = 18 * 32, kManyRows = 256, kManyStep = 128;
+constexpr int kManyThreads = 16 * 32, kManyRows = 256, kManyStep = 128;
+constexpr int kManyDequant = 6;                    // warps that dequantise
 
 template <int HD>
 struct Kv4Many {
@@ -35,6 +36,33 @@ __device__ __forceinline__ uint32_t kv4_dequant2(uint32_t w, __nv_bfloat162 s, _
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ __nv_bfloat162 kv4_bf2(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// two floats in a register pair, an instruction for both
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 f32x2_of(uint64_t v) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 
 // after a failure: the copies and MMAs in flight
 template <int NR>
@@ -71,9 +99,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
   const Kv4Seq& seq = task.seq;
   const int rows = task.rows - task.r0, tiles = rows > 128 ? 2 : 1, n = max(task.n, 0), kvh = task.kvh, total = task.total;
   if (tid == 0) {
-    for (int i = 0; i < NR; i++) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 8); }
+    for (int i = 0; i < NR; i++) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], kManyDequant); }
     for (int i = 0; i < 2; i++) {
-      mbar_init(&k_full[i], 8); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 8); mbar_init(&v_empty[i], 1);
+      mbar_init(&k_full[i], kManyDequant); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], kManyDequant); mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&pv_done[i], 1);
     }
     mbar_init(q_full, 4 * tiles);
@@ -81,7 +109,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
     for (int i = 0; i < 5; i++) s_issued[i] = 0;
     mbar_fence_init();
   }
-  if (warp == 17) {
+  if (warp == 15) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(M::TCOLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -92,7 +120,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
   const WaitCtl wc{S.status, s_abort, P.spin_limit};
   bool ok = true;
 
-  if (warp == 16) {
+  if (warp == 14) {
     // ---------------- pages, two a step; a page behind the last position or that the table does not have is left out
     int r = 0, issued = 0, page = 0;
     uint32_t lap = 1;
@@ -117,7 +145,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       if (++r == NR) { r = 0; lap ^= 1u; }
     }
     if (lane == 0) s_issued[0] = issued;
-  } else if (warp == 17) {
+  } else if (warp == 15) {
     // ---------------- MMA issue: per tile PV of a step, then QK of the next one once PV has read P, which lies over S
     constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);               // bf16 x bf16 -> fp32, 128 rows
     auto qk = [&](int t, int i) {
@@ -166,38 +194,29 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
         }
       }
   } else if (warp >= 8) {
-    // ---------------- dequantise: per page K (tasks of two words: 16 dims of a position), then V (tasks of four words: four dims of eight positions)
+    // ---------------- dequantise: K of a step's two pages, then V, in turns of a warp. K: lanes of a turn take two words each, 16 dims of a position;
+    // V: four words, four dims of eight positions. K's place is free once QK of two steps ago has read it, V's once PV has.
     const int dw = warp - 8;
     int r = 0;
     uint32_t lap = 0;
     for (int i = 0; i < n && ok; i++) {
       const int b = i & 1;
-      if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[b], (uint32_t)((i >> 1) - 1) & 1u, wc, W_EMPTY, 47) &&
-                                                   mbar_wait(&v_empty[b], (uint32_t)((i >> 1) - 1) & 1u, wc, W_EMPTY, 48));
-      for (int h = 0; h < 2 && ok; h++) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[r], lap, wc, W_FULL, 49));
+      const uint32_t before = (uint32_t)((i >> 1) - 1) & 1u;
+      if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[b], before, wc, W_EMPTY, 47));
+      bool none[2], special[2];
+      const uint8_t* rec[2];
+      int left[2], r1 = r;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[r1], lap, wc, W_FULL, 49));
         if (!ok) break;
-        const uint8_t* rec = sm + M::RAW + r * REC;
-        uint8_t *kt = sm + M::K + b * M::KT + h * (kPage * 128), *vt = sm + M::V + (2 * b + h) * M::VT;
-        const int left = total - ((task.unit + i) * kManyStep + h * kPage);      // positions of the page that exist
-        const bool none = s_none[r] != 0 || left <= 0;
-        // V's NaN rows, and what lies behind the last position, become zeros here: every row of P multiplies them
-        unsigned long long bad = 0;
-        if (!none) {
-          const uint32_t a = *reinterpret_cast<const uint32_t*>(rec + (lane >> 4) * C::BLOCK + C::VSZ + (lane & 15) * 4),
-                         c = *reinterpret_cast<const uint32_t*>(rec + (2 + (lane >> 4)) * C::BLOCK + C::VSZ + (lane & 15) * 4);
-          bad = (unsigned long long)__ballot_sync(0xffffffffu, lane < left && !(bflo(a) < INFINITY)) |
-                (unsigned long long)__ballot_sync(0xffffffffu, lane + 32 < left && !(bflo(c) < INFINITY)) << 32;
-        }
-        const bool special = bad != 0 || left < kPage;
-        if (dw == 0 && lane == 0) {
-          s_bad[2 * b + h] = bad;
-          if (h == 0) s_gone[b] = none;
-          else if (none) s_gone[b] = s_gone[b] | 2;
-        }
-        if (!none) {
+        rec[h] = sm + M::RAW + r1 * REC;
+        uint8_t* kt = sm + M::K + b * M::KT + h * (kPage * 128);
+        left[h] = total - ((task.unit + i) * kManyStep + h * kPage);             // positions of the page that exist
+        none[h] = s_none[r1] != 0 || left[h] <= 0;
+        if (!none[h]) {
           auto key = [&](int p, int q) {                         // words 2q, 2q + 1 of position p
-            const uint8_t* blk = rec + (p >> 4) * C::BLOCK;
+            const uint8_t* blk = rec[h] + (p >> 4) * C::BLOCK;
             const uint2 w = *reinterpret_cast<const uint2*>(blk + C::k_word(p & 15, 2 * q));
             const uint32_t sz = *reinterpret_cast<const uint32_t*>(blk + C::KSZ + (p & 15) * 4);
             const __nv_bfloat162 s = kv4_bf2(__byte_perm(sz, sz, 0x1010)), z = kv4_bf2(__byte_perm(sz, sz, 0x3232));
@@ -208,25 +227,46 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
               *reinterpret_cast<uint4*>(row + ((((2 * q + e) & 7) ^ (p & 7)) << 4)) =
                   make_uint4(kv4_dequant2(x[e], s, z), kv4_dequant2(x[e] >> 4, s, z), kv4_dequant2(x[e] >> 8, s, z), kv4_dequant2(x[e] >> 12, s, z));
           };
-          if constexpr (HD == 128) {
-#pragma unroll
-            for (int e = 0; e < 2; e++) key((dw + 8 * e) * 4 + (lane >> 3), lane & 7);
-          } else {
-            key(dw * 8 + (lane >> 2), lane & 3);
-            if (HD == 80 && dw < 2) key(dw * 32 + lane, 4);
-          }
+          constexpr int PT = HD == 128 ? 4 : 8, QN = 32 / PT, TURNS = kPage / PT;          // positions of a turn, tasks of a position's main part
+          for (int j = dw; j < TURNS; j += kManyDequant) key(j * PT + lane / QN, lane & (QN - 1));
+          if (HD == 80 && dw >= 2 && dw < 4) key((dw - 2) * 32 + lane, 4);
         }
-        auto value = [&](int c, int w) {                         // dims 4w .. 4w+3 of positions 8c .. 8c+7
-          const uint8_t* blk = rec + (c >> 1) * C::BLOCK;
+        if (++r1 == NR) { r1 = 0; lap ^= 1u; }
+      }
+      if (!ok) break;
+      // V's NaN rows, and what lies behind the last position, become zeros: every row of P multiplies them
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        unsigned long long bad = 0;
+        if (!none[h]) {
+          const uint32_t a = *reinterpret_cast<const uint32_t*>(rec[h] + (lane >> 4) * C::BLOCK + C::VSZ + (lane & 15) * 4),
+                         c = *reinterpret_cast<const uint32_t*>(rec[h] + (2 + (lane >> 4)) * C::BLOCK + C::VSZ + (lane & 15) * 4);
+          bad = (unsigned long long)__ballot_sync(0xffffffffu, lane < left[h] && !(bflo(a) < INFINITY)) |
+                (unsigned long long)__ballot_sync(0xffffffffu, lane + 32 < left[h] && !(bflo(c) < INFINITY)) << 32;
+        }
+        special[h] = bad != 0 || left[h] < kPage;
+        if (dw == 0 && lane == 0) s_bad[2 * b + h] = bad;
+      }
+      if (dw == 0 && lane == 0) s_gone[b] = (none[0] ? 1 : 0) | (none[1] ? 2 : 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_full[b]);
+      if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[b], before, wc, W_EMPTY, 48));
+      if (!ok) break;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        uint8_t* vt = sm + M::V + (2 * b + h) * M::VT;
+        auto value = [&](int c, int w, auto special_page) {      // dims 4w .. 4w+3 of positions 8c .. 8c+7
+          const uint8_t* blk = rec[h] + (c >> 1) * C::BLOCK;
           uint32_t out[4][4];
 #pragma unroll
           for (int k = 0; k < 4; k++) {
             const int u = (c & 1) * 4 + k;
             const uint32_t x = *reinterpret_cast<const uint32_t*>(blk + C::v_word(u, w));
             uint2 sz = *reinterpret_cast<const uint2*>(blk + C::VSZ + u * 8);
-            if (special) {
-              if (none || 8 * c + 2 * k >= left || !(bflo(sz.x) < INFINITY)) sz.x = 0;
-              if (none || 8 * c + 2 * k + 1 >= left || !(bflo(sz.y) < INFINITY)) sz.y = 0;
+            if (decltype(special_page)::value) {
+              if (8 * c + 2 * k >= left[h] || !(bflo(sz.x) < INFINITY)) sz.x = 0;
+              if (8 * c + 2 * k + 1 >= left[h] || !(bflo(sz.y) < INFINITY)) sz.y = 0;
             }
             const __nv_bfloat162 s = kv4_bf2(__byte_perm(sz.x, sz.y, 0x5410)), z = kv4_bf2(__byte_perm(sz.x, sz.y, 0x7632));
 #pragma unroll
@@ -238,23 +278,26 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
             *reinterpret_cast<uint4*>(vt + d * 128 + ((c ^ (d & 7)) << 4)) = make_uint4(out[e][0], out[e][1], out[e][2], out[e][3]);
           }
         };
-        if (none) {
-          for (int k = tid - 256; k < M::VT / 16; k += 256) *reinterpret_cast<uint4*>(vt + k * 16) = make_uint4(0, 0, 0, 0);
+        if (none[h]) {
+          for (int k = tid - 256; k < M::VT / 16; k += kManyDequant * 32) *reinterpret_cast<uint4*>(vt + k * 16) = make_uint4(0, 0, 0, 0);
         } else {
           // a phase of eight lanes stores to eight chunks; four chunks' lanes read words of different bank groups
           const int ci = (lane >> 1) & 3, wi = (lane & 1) | (lane >> 3) << 1;
           constexpr int NG = C::MAIN / 32;                       // groups of eight words
-          if (dw < 2 * NG) value(4 * (dw & 1) + ci, 8 * (((dw >> 1) + ci) & (NG - 1)) + wi);
-          if (HD == 80 && dw == 7) value((lane >> 1) & 7, 16 + ((lane & 1) | (lane >> 4) << 1));
+          auto turns = [&](auto special_page) {
+            for (int j = (dw + 4 * h) % kManyDequant; j < 2 * NG; j += kManyDequant) value(4 * (j & 1) + ci, 8 * (((j >> 1) + ci) & (NG - 1)) + wi, special_page);
+            if (HD == 80 && dw == (h ? 5 : 4)) value((lane >> 1) & 7, 16 + ((lane & 1) | (lane >> 4) << 1), special_page);
+          };
+          if (special[h]) turns(std::true_type());
+          else turns(std::false_type());
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&raw_empty[r]);
-        if (++r == NR) { r = 0; lap ^= 1u; }
+        if (++r == NR) r = 0;
       }
-      if (!ok) break;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) { mbar_arrive(&k_full[b]); mbar_arrive(&v_full[b]); }
+      if (lane == 0) mbar_arrive(&v_full[b]);
     }
   } else if (warp >> 2 < tiles) {
     // ---------------- softmax of tile t: thread = row
@@ -283,31 +326,44 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], (uint32_t)i & 1u, wc, W_FULL, 50));
       if (!ok) break;
       tc_fence_after();
-      // the step's V is dequantised by now or soon: its flags are needed only where something is special
       const int p0 = (task.unit + i) * kManyStep, gone = s_gone[i & 1];
-      const bool edge = p0 + kManyStep > seq.cached || gone;
-      float mx = -INFINITY;
+      const unsigned long long bad0 = s_bad[2 * (i & 1)], bad1 = s_bad[2 * (i & 1) + 1];
+      const bool edge = p0 + kManyStep > seq.cached || gone || (bad0 | bad1) != 0;
+      if (edge) {                                                // what is not seen becomes -inf in place; apart from the hot loops, which have no branches
+#pragma unroll 1
+        for (int c = 0; c < 8; c++) {
+          uint32_t x[16];
+          tc_ld16(ts + c * 16, x);
+          tc_ld_wait();
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        uint32_t v[32];
-        tc_ld32(ts + c * 32, v);
-        tc_ld_wait();
-        if (edge) {
-#pragma unroll
-          for (int e = 0; e < 32; e++) {
-            const int tp = p0 + c * 32 + e, j = tp - seq.cached;
-            bool see = tp < total && !(gone >> (c >> 1) & 1);
+          for (int e = 0; e < 16; e++) {
+            const int tp = p0 + c * 16 + e, j = tp - seq.cached;
+            bool see = tp < total && !(gone >> (c >> 2) & 1);
             if (see && j >= 0) see = mask ? j < P.mask_ld && mask[j] != 0 : j <= mq;
-            if (!see) v[e] = 0xff800000u;
+            if (!see) x[e] = 0xff800000u;
+            else if (((c < 4 ? bad0 : bad1) >> (16 * (c & 3) + e)) & 1) l = __uint_as_float(0x7fc00000u);      // sees a row of V that is NaN
           }
           __syncwarp();
-          tc_st32(ts + c * 32, v);
+          tc_st16(ts + c * 16, x);
         }
-#pragma unroll
-        for (int e = 0; e < 32; e++) mx = fmaxf(mx, __uint_as_float(v[e]));
+        tc_st_wait();
       }
-      if (edge) tc_st_wait();
-      const float top = mx * cs;
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      uint32_t v[2][32];                                         // a piece of 32 columns is loaded while the one before it is worked on
+      tc_ld32(ts, v[0]);
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        uint32_t(&x)[32] = v[c & 1];
+        tc_ld_wait();
+        if (c < 3) tc_ld32(ts + (c + 1) * 32, v[(c + 1) & 1]);
+#pragma unroll
+        for (int e = 0; e < 32; e += 8)
+#pragma unroll
+          for (int k = 0; k < 4; k++) mx[k] = max3(mx[k], __uint_as_float(x[e + 2 * k]), __uint_as_float(x[e + 2 * k + 1]));
+      }
+      uint32_t u[2][16];                                         // again, in pieces of 16
+      tc_ld16(ts, u[0]);
+      const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * cs;
       if (__any_sync(0xffffffffu, top > m + 8.f)) {
         const float mn = fmaxf(m, top), corr = ex2(m - mn);
         if (i > 0) {                                             // O as the steps before left it
@@ -327,28 +383,26 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
         m = mn;
         l *= corr;
       }
-      const unsigned long long bad0 = s_bad[2 * (i & 1)], bad1 = s_bad[2 * (i & 1) + 1];
+      const uint64_t cs2 = f32x2(cs, cs), m2 = f32x2(-m, -m);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        uint32_t v[32], o[16];
-        tc_ld32(ts + c * 32, v);
+      for (int c = 0; c < 8; c++) {
+        uint32_t(&x)[16] = u[c & 1];
+        uint32_t o[8];
         tc_ld_wait();
-        float s0 = 0.f, s1 = 0.f;
+        if (c < 7) tc_ld16(ts + (c + 1) * 16, u[(c + 1) & 1]);
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const float a = ex2(fmaf(__uint_as_float(v[2 * e]), cs, -m)), d = ex2(fmaf(__uint_as_float(v[2 * e + 1]), cs, -m));
-          s0 += a;
-          s1 += d;
+        for (int e = 0; e < 8; e++) {
+          const float2 y = f32x2_of(fma_f32x2((uint64_t)x[2 * e] | (uint64_t)x[2 * e + 1] << 32, cs2, m2));
+          const float a = ex2(y.x), d = ex2(y.y);
+          sum[e & 1] = add_f32x2(sum[e & 1], f32x2(a, d));
           asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[e]) : "f"(d), "f"(a));
         }
-        l += s0 + s1;
-        if (bad0 | bad1) {                                       // a row of V that is NaN, for the rows that see it
-          const uint32_t bad = (uint32_t)((c < 2 ? bad0 : bad1) >> (32 * (c & 1)));
-#pragma unroll
-          for (int e = 0; e < 32; e++)
-            if ((bad >> e & 1) && v[e] != 0xff800000u) l = __uint_as_float(0x7fc00000u);
-        }
-        tc_st16(ts + c * 16, o);
+        tc_st8v(ts + c * 8, o);
+      }
+      {
+        const float2 y = f32x2_of(add_f32x2(sum[0], sum[1]));
+        l += y.x + y.y;
       }
       tc_st_wait();
       tc_fence_before();
@@ -391,7 +445,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 17) {
+  if (warp == 15) {
     if (*s_abort) many_drain<NR>(raw_full, s_full, pv_done, s_issued);
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(M::TCOLS));
   }
