@@ -109,11 +109,20 @@ cudaError_t launch_few(Kv4Attend p, const Kv4Geometry& g, cudaStream_t st) {
     return launch_pdl(kv4_join<HD, F::ROWS, F::U, 8>, dim3((unsigned)g.groups, (unsigned)p.S.nkv, F::ROWS), dim3(256), 0, st, p);
   return launch_pdl(kv4_join<HD, F::ROWS, F::U, 1>, dim3((unsigned)g.groups, (unsigned)p.S.nkv, F::ROWS / 8), dim3(256), 0, st, p);
 }
+// kv4_attn_many deals its registers out anew and counts on 128 a thread at launch
+template <int HD>
+bool configured_many() {
+  static int regs = 0;
+  cudaFuncAttributes a;
+  if (!regs && cudaFuncGetAttributes(&a, kv4_attn_many<HD>) == cudaSuccess) regs = a.numRegs;
+  return regs == 128;
+}
 template <int HD>
 cudaError_t launch_many(Kv4Attend p, const Kv4Geometry& g, cudaStream_t st) {
   static bool done[64] = {};
   p.nsplit = 1; p.slots = g.slots; p.chunk = g.chunk;
   if (g.groups > 0x7fffffff || g.ctas > 0x7fffffff) return cudaErrorInvalidValue;
+  if (g.groups > 0 && !configured_many<HD>()) return cudaErrorInvalidConfiguration;
   cudaError_t e = configure_few(kv4_attn_many<HD>, Kv4Many<HD>::TOTAL, done);
   if (e == cudaSuccess) e = launch_pdl(kv4_attn_many<HD>, dim3((unsigned)g.ctas), dim3(kManyThreads), (size_t)Kv4Many<HD>::TOTAL, st, p);
   if (e == cudaSuccess && g.slots)

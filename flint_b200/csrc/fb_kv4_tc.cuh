@@ -120,6 +120,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
   const WaitCtl wc{S.status, s_abort, P.spin_limit};
   bool ok = true;
 
+  // The block's 512 x 128 registers are dealt out anew, 256 x 176 + 256 x 80: the softmax keeps a row's 128 scores
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
   if (warp == 14) {
     // ---------------- pages, two a step; a page behind the last position or that the table does not have is left out
     int r = 0, issued = 0, page = 0;
@@ -148,31 +151,34 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
   } else if (warp == 15) {
     // ---------------- MMA issue: per tile PV of a step, then QK of the next one once PV has read P, which lies over S
     constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);               // bf16 x bf16 -> fp32, 128 rows
-    auto qk = [&](int t, int i) {
-      const int b = i & 1;
+    const uint64_t q0 = tc_desc(smem_u32(sm + M::Q)), k0 = tc_desc(smem_u32(sm + M::K)), v0 = tc_desc(smem_u32(sm + M::V));
+    auto qk = [&](auto tile, int i) {
+      constexpr int t = decltype(tile)::value;
       if (elect_one()) {
-        const uint64_t qa = tc_desc(smem_u32(sm + M::Q + t * M::QT)), kb = tc_desc(smem_u32(sm + M::K + b * M::KT));
+        const uint64_t kb = k0 + (uint64_t)((i & 1) * (M::KT >> 4));
 #pragma unroll
         for (int k = 0; k < KS; k++) {
+          constexpr uint32_t id = idesc | ((128u >> 3) << 17);
           const uint64_t off = (uint64_t)(((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4);
-          tc_mma_ss(tmem + M::T_S + t * 128, qa + off, kb + off, idesc | ((128u >> 3) << 17), k ? 1u : 0u);
+          tc_mma_ss(tmem + M::T_S + t * 128, q0 + (uint64_t)(t * (M::QT >> 4)) + off, kb + off, id, k ? 1u : 0u);
         }
         tc_commit(&s_full[t]);
-        if (t == tiles - 1) tc_commit(&k_empty[b]);
+        if (t == tiles - 1) tc_commit(&k_empty[i & 1]);
       }
       __syncwarp();
       if (lane == 0) s_issued[1 + t] = i + 1;
     };
-    auto pv = [&](int t, int i) {
-      const int b = i & 1;
+    auto pv = [&](auto tile, int i) {
+      constexpr int t = decltype(tile)::value;
       if (elect_one()) {
-        const uint64_t vb = tc_desc(smem_u32(sm + M::V + b * 2 * M::VT));
+        const uint64_t vb = v0 + (uint64_t)((i & 1) * (M::VT >> 3));
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-          tc_mma_ts(tmem + M::T_O + t * HD, tmem + M::T_S + t * 128 + k * 8, vb + (uint64_t)(((k >> 2) * M::VT + (k & 3) * 32) >> 4),
-                    idesc | ((uint32_t)(HD >> 3) << 17), i || k ? 1u : 0u);
+        for (int k = 0; k < 8; k++) {
+          constexpr uint32_t id = idesc | ((uint32_t)(HD >> 3) << 17);
+          tc_mma_ts(tmem + M::T_O + t * HD, tmem + M::T_S + t * 128 + k * 8, vb + (uint64_t)(((k >> 2) * M::VT + (k & 3) * 32) >> 4), id, i || k ? 1u : 0u);
+        }
         tc_commit(&pv_done[t]);
-        if (t == tiles - 1) tc_commit(&v_empty[b]);
+        if (t == tiles - 1) tc_commit(&v_empty[i & 1]);
       }
       __syncwarp();
       if (lane == 0) s_issued[3 + t] = i + 1;
@@ -182,18 +188,24 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       tc_fence_after();
       return ok;
     };
-    if (n > 0 && wait(q_full, 0, 41) && wait(&k_full[0], 0, 42))
-      for (int t = 0; t < tiles; t++) qk(t, 0);
-    for (int i = 0; i < n && ok; i++)
-      for (int t = 0; t < tiles && ok; t++) {
-        if (!wait(&p_full[t], i, 43) || (t == 0 && !wait(&v_full[i & 1], i >> 1, 44))) break;
-        pv(t, i);
-        if (i + 1 < n) {
-          if ((t == 0 && !wait(&k_full[(i + 1) & 1], (i + 1) >> 1, 45)) || !wait(&pv_done[t], i, 46)) break;
-          qk(t, i + 1);
-        }
-      }
-  } else if (warp >= 8) {
+    const std::integral_constant<int, 0> first;
+    const std::integral_constant<int, 1> second;
+    if (n > 0 && wait(q_full, 0, 41) && wait(&k_full[0], 0, 42)) {
+      qk(first, 0);
+      if (tiles > 1) qk(second, 0);
+    }
+    auto turn = [&](auto tile, int i) {
+      constexpr int t = decltype(tile)::value;
+      if (!wait(&p_full[t], i, 43) || (t == 0 && !wait(&v_full[i & 1], i >> 1, 44))) return;
+      pv(tile, i);
+      if (i + 1 == n || (t == 0 && !wait(&k_full[(i + 1) & 1], (i + 1) >> 1, 45)) || !wait(&pv_done[t], i, 46)) return;
+      qk(tile, i + 1);
+    };
+    for (int i = 0; i < n && ok; i++) {
+      turn(first, i);
+      if (tiles > 1 && ok) turn(second, i);
+    }
+  } else {
     // ---------------- dequantise: K of a step's two pages, then V, in turns of a warp. K: lanes of a turn take two words each, 16 dims of a position;
     // V: four words, four dims of eight positions. K's place is free once QK of two steps ago has read it, V's once PV has.
     const int dw = warp - 8;
@@ -215,21 +227,29 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
         left[h] = total - ((task.unit + i) * kManyStep + h * kPage);             // positions of the page that exist
         none[h] = s_none[r1] != 0 || left[h] <= 0;
         if (!none[h]) {
-          auto key = [&](int p, int q) {                         // words 2q, 2q + 1 of position p
+          auto key = [&](int p, int w0, auto words) {            // words w0 .. of position p
+            constexpr int NWD = decltype(words)::value;
             const uint8_t* blk = rec[h] + (p >> 4) * C::BLOCK;
-            const uint2 w = *reinterpret_cast<const uint2*>(blk + C::k_word(p & 15, 2 * q));
+            uint32_t x[NWD];
+            if (NWD == 4) {
+              const uint4 w = *reinterpret_cast<const uint4*>(blk + C::k_word(p & 15, w0));
+              x[0] = w.x; x[1] = w.y; x[NWD - 2] = w.z; x[NWD - 1] = w.w;
+            } else {
+              const uint2 w = *reinterpret_cast<const uint2*>(blk + C::k_word(p & 15, w0));
+              x[0] = w.x; x[1] = w.y;
+            }
             const uint32_t sz = *reinterpret_cast<const uint32_t*>(blk + C::KSZ + (p & 15) * 4);
             const __nv_bfloat162 s = kv4_bf2(__byte_perm(sz, sz, 0x1010)), z = kv4_bf2(__byte_perm(sz, sz, 0x3232));
-            uint8_t* row = kt + (q >> 2) * (kManyStep * 128) + p * 128;
-            const uint32_t x[2] = {w.x, w.y};
+            uint8_t* row = kt + (w0 >> 3) * (kManyStep * 128) + p * 128;
 #pragma unroll
-            for (int e = 0; e < 2; e++)
-              *reinterpret_cast<uint4*>(row + ((((2 * q + e) & 7) ^ (p & 7)) << 4)) =
+            for (int e = 0; e < NWD; e++)
+              *reinterpret_cast<uint4*>(row + ((((w0 + e) & 7) ^ (p & 7)) << 4)) =
                   make_uint4(kv4_dequant2(x[e], s, z), kv4_dequant2(x[e] >> 4, s, z), kv4_dequant2(x[e] >> 8, s, z), kv4_dequant2(x[e] >> 12, s, z));
           };
-          constexpr int PT = HD == 128 ? 4 : 8, QN = 32 / PT, TURNS = kPage / PT;          // positions of a turn, tasks of a position's main part
-          for (int j = dw; j < TURNS; j += kManyDequant) key(j * PT + lane / QN, lane & (QN - 1));
-          if (HD == 80 && dw >= 2 && dw < 4) key((dw - 2) * 32 + lane, 4);
+          constexpr int QN = C::MAIN / 32, PT = 32 / QN, TURNS = kPage / PT;             // lanes of a position, positions of a turn
+          for (int j = (dw + 4 * h) % kManyDequant; j < TURNS; j += kManyDequant)
+            key(j * PT + lane / QN, 4 * (lane & (QN - 1)), std::integral_constant<int, 4>());
+          if (HD == 80 && dw >= 2 && dw < 4) key((dw - 2) * 32 + lane, 8, std::integral_constant<int, 2>());
         }
         if (++r1 == NR) { r1 = 0; lap ^= 1u; }
       }
@@ -299,7 +319,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       __syncwarp();
       if (lane == 0) mbar_arrive(&v_full[b]);
     }
-  } else if (warp >> 2 < tiles) {
+  }
+  } else {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+  if (warp >> 2 < tiles) {
     // ---------------- softmax of tile t: thread = row
     const int t = warp >> 2, row = tid & 127, lr = t * 128 + row, R = P.R;
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = tl + M::T_S + t * 128, to = tl + M::T_O + t * HD;
@@ -321,49 +344,47 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
     }
     const float cs = fmaxf(fabsf(P.scale), 1e-30f);              // not zero: a score that is not seen stays -inf
     const uint8_t* mask = P.amask ? P.amask + (size_t)(seq.first + mq) * P.mask_ld : nullptr;
+    const int m_first = (task.r0 + min(t * 128 + (warp & 3) * 32, rows - 1)) / R;          // the warp's first token: what it sees, all rows see
     float m = -1e30f, l = 0.f;
     for (int i = 0; i < n; i++) {
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], (uint32_t)i & 1u, wc, W_FULL, 50));
       if (!ok) break;
       tc_fence_after();
+      uint32_t v[4][32];                                         // the row's scores, then its probabilities, stay in registers
+#pragma unroll
+      for (int c = 0; c < 4; c++) tc_ld32(ts + c * 32, v[c]);
       const int p0 = (task.unit + i) * kManyStep, gone = s_gone[i & 1];
       const unsigned long long bad0 = s_bad[2 * (i & 1)], bad1 = s_bad[2 * (i & 1) + 1];
-      const bool edge = p0 + kManyStep > seq.cached || gone || (bad0 | bad1) != 0;
-      if (edge) {                                                // what is not seen becomes -inf in place; apart from the hot loops, which have no branches
+      tc_ld_wait();
+      if (p0 + kManyStep > (mask ? seq.cached : min(total, seq.cached + m_first + 1)) || gone || (bad0 | bad1)) {
+        // what is not seen becomes -inf
+        uint32_t vis[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const int q0 = p0 + 32 * c, lim = (mask ? min(total, seq.cached) : min(total, seq.cached + mq + 1)) - q0;
+          vis[c] = lim >= 32 ? 0xffffffffu : (lim > 0 ? (1u << lim) - 1u : 0u);
+          if (mask && lim < 32)
 #pragma unroll 1
-        for (int c = 0; c < 8; c++) {
-          uint32_t x[16];
-          tc_ld16(ts + c * 16, x);
-          tc_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            const int tp = p0 + c * 16 + e, j = tp - seq.cached;
-            bool see = tp < total && !(gone >> (c >> 2) & 1);
-            if (see && j >= 0) see = mask ? j < P.mask_ld && mask[j] != 0 : j <= mq;
-            if (!see) x[e] = 0xff800000u;
-            else if (((c < 4 ? bad0 : bad1) >> (16 * (c & 3) + e)) & 1) l = __uint_as_float(0x7fc00000u);      // sees a row of V that is NaN
-          }
-          __syncwarp();
-          tc_st16(ts + c * 16, x);
+            for (int j = max(0, q0 - seq.cached); j < min(min(total, q0 + 32) - seq.cached, P.mask_ld); j++)
+              vis[c] |= (mask[j] != 0 ? 1u : 0u) << (seq.cached + j - q0);
+          if (gone >> (c >> 1) & 1) vis[c] = 0;
+          if (vis[c] & (uint32_t)((c < 2 ? bad0 : bad1) >> (32 * (c & 1)))) l = __uint_as_float(0x7fc00000u);       // sees a row of V that is NaN
         }
-        tc_st_wait();
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+          for (int e = 0; e < 32; e++)
+            if (!(vis[c] & 1u << e)) v[c][e] = 0xff800000u;
+        __syncwarp();
       }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      uint32_t v[2][32];                                         // a piece of 32 columns is loaded while the one before it is worked on
-      tc_ld32(ts, v[0]);
+      float mx[8];
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        uint32_t(&x)[32] = v[c & 1];
-        tc_ld_wait();
-        if (c < 3) tc_ld32(ts + (c + 1) * 32, v[(c + 1) & 1]);
+      for (int k = 0; k < 8; k++) mx[k] = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 32; e += 8)
+      for (int c = 0; c < 4; c++)
 #pragma unroll
-          for (int k = 0; k < 4; k++) mx[k] = max3(mx[k], __uint_as_float(x[e + 2 * k]), __uint_as_float(x[e + 2 * k + 1]));
-      }
-      uint32_t u[2][16];                                         // again, in pieces of 16
-      tc_ld16(ts, u[0]);
-      const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * cs;
+        for (int e = 0; e < 32; e += 2) mx[(e >> 1) & 7] = max3(mx[(e >> 1) & 7], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
+      const float top = fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[4]), max3(mx[5], mx[6], mx[7])) * cs;
       if (__any_sync(0xffffffffu, top > m + 8.f)) {
         const float mn = fmaxf(m, top), corr = ex2(m - mn);
         if (i > 0) {                                             // O as the steps before left it
@@ -371,37 +392,34 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
           if (!ok) break;
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < HD; c += 16) {
-            uint32_t v[16];
-            tc_ld16(to + c, v);
+          for (int c = 0; c < HD; c += 8) {
+            uint32_t x[8];
+            tc_ld8(to + c, x);
             tc_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * corr);
-            tc_st16(to + c, v);
+            for (int e = 0; e < 8; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * corr);
+            tc_st8v(to + c, x);
           }
         }
         m = mn;
         l *= corr;
       }
       const uint64_t cs2 = f32x2(cs, cs), m2 = f32x2(-m, -m);
-      uint64_t sum[2] = {0, 0};
+      uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int c = 0; c < 8; c++) {
-        uint32_t(&x)[16] = u[c & 1];
-        uint32_t o[8];
-        tc_ld_wait();
-        if (c < 7) tc_ld16(ts + (c + 1) * 16, u[(c + 1) & 1]);
+      for (int c = 0; c < 4; c++) {
+        uint32_t o[16];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float2 y = f32x2_of(fma_f32x2((uint64_t)x[2 * e] | (uint64_t)x[2 * e + 1] << 32, cs2, m2));
+        for (int e = 0; e < 16; e++) {
+          const float2 y = f32x2_of(fma_f32x2(f32x2(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), cs2, m2));
           const float a = ex2(y.x), d = ex2(y.y);
-          sum[e & 1] = add_f32x2(sum[e & 1], f32x2(a, d));
+          sum[e & 3] = add_f32x2(sum[e & 3], f32x2(a, d));
           asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[e]) : "f"(d), "f"(a));
         }
-        tc_st8v(ts + c * 8, o);
+        tc_st16(ts + c * 16, o);
       }
       {
-        const float2 y = f32x2_of(add_f32x2(sum[0], sum[1]));
+        const float2 y = f32x2_of(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])));
         l += y.x + y.y;
       }
       tc_st_wait();
@@ -442,6 +460,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       }
       if (w && live) *reinterpret_cast<float2*>(w + HD) = make_float2(m, l);
     }
+  }
   }
   tc_fence_before();
   __syncthreads();
