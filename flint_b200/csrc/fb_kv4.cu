@@ -1,10 +1,6 @@
 // extern "C" entry points of the 4-bit paged K/V cache: append, attention, read-back, moves.
 // No torch types, no CPU fallback: a failed CUDA call or an unsupported shape is an error code.
 #include <string.h>
-#include <stdlib.h>
-#include <stdio.h>
-#include <stdlib.h>
-#include <stdio.h>
 
 #include "../../include/flint_b200.h"
 #include "fb_ctx.hpp"
@@ -15,6 +11,7 @@ using namespace fb;
 
 namespace {
 
+constexpr int kFewRows = 64;
 constexpr int kFewWarps = 7;                       // that compute, of a CTA of kv4_attn_few; an SM holds two CTAs
 
 int device_sms(int dev) {
@@ -50,23 +47,34 @@ int take_seqs(const fb_kv4_seqs* s, int rows_of_tokens, Kv4Seqs& S) {
 }
 int done(cudaError_t e) { return e == cudaSuccess ? FB_OK : FB_ERR_CUDA; }
 
-// How an attention of few rows is cut. rows: query rows of a group; groups: of all sequences, at most; ctas: of a grid without clusters, at most.
-// A group's positions are shared by a cluster (one launch) while a warp of a cluster of eight has no more than six units; by as many CTAs as the GPU holds and a
-// second launch that joins them, beyond that. (With one CTA of 16-row groups per SM the GPU holds 15 clusters of 8, but 36 of 4.) Microseconds, one sequence, eight kv heads, cluster / second launch: 1000 positions 5.5 / 8.2, 4000 6.7 / 8.5,
-// 32768 20.5 / 13.1 (heads of 80). Of a batch no positions are shared until a warp would have more than 12 units: 48 sequences of up to 2000
-// positions 17.8 / 22.7, 24 of up to 8000 51 / 18.3 (over 148 parts; over 296 22.1).
+// How an attention is cut. rows: query rows of a group; groups: of all sequences, at most; ctas: of a grid without clusters, at most.
+// Up to kFewRows query rows a kv head: kv4_attn_few in groups of 8 or 16 rows, which dequantise the cache anew for each group. More: kv4_attn_many. Microseconds, few /
+// many: 16 tokens of 4 heads (64 rows) behind 1024 positions 9.9 / 13.5, behind 4000 14.5 / 17.5, 12 (48 rows) behind 8000 24.2 / 23.9; 26 tokens (104 rows) behind
+// 1024 13.5 / 13.2, behind 8000 44 / 26; 61 (244 rows) behind 3001 46 / 28.
+// Few: a group's positions are shared by a cluster (one launch) while a warp of a cluster of eight has no more than six units; by as many CTAs as the GPU holds and a
+// second launch that joins them, beyond that. (With one CTA of 16-row groups per SM the GPU holds 15 clusters of 8, but 36 of 4.) One sequence, eight
+// kv heads, cluster / second launch: 1000 positions 5.5 / 8.2, 4000 6.7 / 8.5, 32768 20.5 / 13.1 (heads of 80). Of a batch no positions are shared until a
+// warp would have more than 12 units: 48 sequences of up to 2000 positions 17.8 / 22.7, 24 of up to 8000 51 / 18.3 (over 148 parts; over 296 22.1).
+// Many: a step of 128 positions takes 2.5 us (1.6 with one tile of rows), a task about two steps more, the second launch 5 us and what the partials take to
+// write and read; the number of parts with the smallest sum is taken. 1000 tokens behind 7011 positions, 160 items on 148 SMs: whole 253, four
+// parts 216; 128 items: whole 160, two parts 197. 61-node tree, eight items: whole 71, eight parts 28.4, 24 parts 42.
 struct Kv4Geometry { int rows; int64_t groups, ctas; int nsplit, slots, chunk; };
 Kv4Geometry few_geometry(int n_seq, int n_tokens, int nkv, int r, int max_new, int max_len, int sms) {
   Kv4Geometry g{(int64_t)max_new * r <= 8 ? 8 : 16, 0, 0, 1, 0, 8};
-  int from = 65, slots = -1, chunk = 2;
-  if (getenv("KV4")) sscanf(getenv("KV4"), "%d,%d,%d", &from, &slots, &chunk);
-  if ((int64_t)max_new * r >= from) g.rows = kManyRows;
+  if ((int64_t)max_new * r > kFewRows) g.rows = kManyRows;
   g.groups = n_seq == 1 ? ((int64_t)n_tokens * r + g.rows - 1) / g.rows : (int64_t)n_tokens * r / g.rows + n_seq;
   const int64_t units = ((int64_t)max_len + 31) / 32, items = g.groups * nkv;
   if (g.rows == kManyRows) {
-    g.chunk = chunk;
-    if (items * 3 < sms * 2) g.slots = sms;
-    if (slots >= 0) g.slots = slots;
+    g.chunk = 1;
+    const int64_t steps = ((int64_t)max_len + kManyStep - 1) / kManyStep;
+    const double step_us = (int64_t)max_new * r > 128 ? 2.5 : 1.6;
+    double best = 0;
+    for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24}) {
+      if (parts > steps || (parts > 1 && items * parts > 3 * sms)) break;
+      const int64_t per = (steps + parts - 1) / parts, tasks = items * ((steps + per - 1) / per);
+      const double us = (double)((tasks + sms - 1) / sms) * (double)(per + 2) * step_us + (parts > 1 ? 5.0 + (double)tasks * kManyRows * 1056 / 3e6 : 0.0);
+      if (parts == 1 || us < best) { best = us; g.slots = parts > 1 ? (int)(items * parts) : 0; }
+    }
   } else if (n_seq == 1) {
     while (g.nsplit < 8 && items * g.nsplit * 2 <= (g.nsplit == 4 ? sms * 2 / 3 : sms) && units >= g.nsplit * 2 * 4) g.nsplit *= 2;
     if (units > (int64_t)6 * kFewWarps * g.nsplit && items * g.nsplit <= sms) { g.nsplit = 1; g.slots = 2 * sms; }
@@ -263,8 +271,8 @@ int kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n_he
   }
 }
 
-// one sequence is split over clusterless CTAs only while its row groups are fewer than the SMs
-size_t kv4_attend_most(int n_kv_head, int head_dim, int sms) { return (size_t)(2 * sms + n_kv_head) * kManyRows * (head_dim + 4) * 4; }
+// one sequence: few rows are split while their groups are fewer than the SMs, into two parts an SM more; many rows into three an SM at most
+size_t kv4_attend_most(int n_kv_head, int head_dim, int sms) { return (size_t)(5 * sms) * kManyRows * (head_dim + 4) * 4; }
 
 size_t fb_kv4_attend_bytes(const fb_kv4_seqs* s, int32_t n_head, int32_t max_new, int32_t max_len) {
   if (!s || s->n_kv_head < 1 || s->n_kv_head > 65535 || n_head < 1 || n_head % s->n_kv_head || max_new < 1 || max_len < 1 || s->n_seq < 0) return 0;

@@ -22,9 +22,9 @@ template <int HD>
 struct Kv4Many {
   static constexpr int REC = Kv4<HD>::REC, NB = HD == 64 ? 1 : 2;           // blocks of 64 dims of a K-major tile
   static constexpr int QT = NB * 128 * 128, KT = NB * kManyStep * 128, VT = HD * 128;      // bytes: Q tile, K step, V page
-  static constexpr int NR = 3;                                              // pages in flight
+  static constexpr int NR = 4;                                              // pages: two being dequantised, two on their way
   static constexpr int Q = 0, K = Q + 2 * QT, V = K + 2 * KT, RAW = V + 4 * VT, BAR = RAW + NR * REC;
-  static constexpr int TOTAL = BAR + 256 + 1024;                            // + slack to align the base
+  static constexpr int BARS = 2 * NR + 15, TOTAL = BAR + BARS * 8 + 4 * 8 + (2 + 5 + NR + 2) * 4;       // barriers, then what stands behind them in the kernel
   static constexpr int T_S = 0, T_O = 256, TCOLS = 512;                     // tensor memory columns: two S / P, two O
   static_assert(TOTAL <= 227 * 1024 && T_O + 2 * HD <= TCOLS && QT % 1024 == 0 && VT % 1024 == 0 && RAW % 16 == 0 && REC % 16 == 0, "plan");
 };
@@ -80,12 +80,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
   using C = Kv4<HD>;
   using M = Kv4Many<HD>;
   constexpr int NR = M::NR, REC = M::REC, KS = HD / 16;
-  extern __shared__ __align__(1024) uint8_t tsm_raw[];
-  uint8_t* sm = tsm_raw + ((1024u - (smem_u32(tsm_raw) & 1023u)) & 1023u);
+  extern __shared__ __align__(1024) uint8_t many_sm[];                // the swizzle is a function of the address: tiles start on 1024-byte boundaries
+  uint8_t* const sm = many_sm;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + M::BAR);
   uint64_t *raw_full = bars, *raw_empty = raw_full + NR, *k_full = raw_empty + NR, *k_empty = k_full + 2, *v_full = k_empty + 2, *v_empty = v_full + 2,
            *s_full = v_empty + 2, *p_full = s_full + 2, *pv_done = p_full + 2, *q_full = pv_done + 2;
-  unsigned long long* s_bad = reinterpret_cast<unsigned long long*>(q_full + 1);       // [2 steps][2 pages] positions whose V is NaN
+  unsigned long long* s_bad = reinterpret_cast<unsigned long long*>(bars + M::BARS);   // [2 steps][2 pages] positions whose V is NaN
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_bad + 4);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   volatile int* s_issued = s_abort + 1;                          // [5] pages, QK of tiles 0 and 1, PV of tiles 0 and 1
@@ -208,116 +208,125 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
   } else {
     // ---------------- dequantise: K of a step's two pages, then V, in turns of a warp. K: lanes of a turn take two words each, 16 dims of a position;
     // V: four words, four dims of eight positions. K's place is free once QK of two steps ago has read it, V's once PV has.
+    // The turns of both pages are dealt out to the warps together. (Unrolled, they do not fit 80 registers: 160 us of 1000 tokens behind 7011 became 204.)
     const int dw = warp - 8;
+    constexpr int QN = C::MAIN / 32, PT = 32 / QN, KTURNS = kPage / PT, VTURNS = C::MAIN / 16;       // lanes of a position, positions of a turn, turns of a page
+    auto key = [&](const uint8_t* rec, uint8_t* kt, int p, int w0, auto words) {           // words w0 .. of position p
+      constexpr int NWD = decltype(words)::value;
+      const uint8_t* blk = rec + (p >> 4) * C::BLOCK;
+      uint32_t x[NWD];
+      if (NWD == 4) {
+        const uint4 w = *reinterpret_cast<const uint4*>(blk + C::k_word(p & 15, w0));
+        x[0] = w.x; x[1] = w.y; x[NWD - 2] = w.z; x[NWD - 1] = w.w;
+      } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(blk + C::k_word(p & 15, w0));
+        x[0] = w.x; x[1] = w.y;
+      }
+      const uint32_t sz = *reinterpret_cast<const uint32_t*>(blk + C::KSZ + (p & 15) * 4);
+      const __nv_bfloat162 s = kv4_bf2(__byte_perm(sz, sz, 0x1010)), z = kv4_bf2(__byte_perm(sz, sz, 0x3232));
+      uint8_t* row = kt + (w0 >> 3) * (kManyStep * 128) + p * 128;
+#pragma unroll
+      for (int e = 0; e < NWD; e++)
+        *reinterpret_cast<uint4*>(row + ((((w0 + e) & 7) ^ (p & 7)) << 4)) =
+            make_uint4(kv4_dequant2(x[e], s, z), kv4_dequant2(x[e] >> 4, s, z), kv4_dequant2(x[e] >> 8, s, z), kv4_dequant2(x[e] >> 12, s, z));
+    };
+    auto value = [&](const uint8_t* rec, uint8_t* vt, int c, int w, int left, auto special) {        // dims 4w .. 4w+3 of positions 8c .. 8c+7
+      const uint8_t* blk = rec + (c >> 1) * C::BLOCK;
+      uint32_t out[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int u = (c & 1) * 4 + k;
+        const uint32_t x = *reinterpret_cast<const uint32_t*>(blk + C::v_word(u, w));
+        uint2 sz = *reinterpret_cast<const uint2*>(blk + C::VSZ + u * 8);
+        if (decltype(special)::value) {
+          if (8 * c + 2 * k >= left || !(bflo(sz.x) < INFINITY)) sz.x = 0;
+          if (8 * c + 2 * k + 1 >= left || !(bflo(sz.y) < INFINITY)) sz.y = 0;
+        }
+        const __nv_bfloat162 s = kv4_bf2(__byte_perm(sz.x, sz.y, 0x5410)), z = kv4_bf2(__byte_perm(sz.x, sz.y, 0x7632));
+#pragma unroll
+        for (int e = 0; e < 4; e++) out[e][k] = kv4_dequant2(x >> (4 * e), s, z);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int d = 4 * w + e;
+        *reinterpret_cast<uint4*>(vt + d * 128 + ((c ^ (d & 7)) << 4)) = make_uint4(out[e][0], out[e][1], out[e][2], out[e][3]);
+      }
+    };
+    // a V turn: a phase of eight lanes stores to eight chunks; four chunks' lanes read words of different bank groups
+    const int ci = (lane >> 1) & 3, wi = (lane & 1) | (lane >> 3) << 1;
+    auto chunk_of = [&](int j) { return 4 * (j & 1) + ci; };
+    auto word_of = [&](int j) { return 8 * (((j >> 1) + ci) & (VTURNS / 2 - 1)) + wi; };
+    const std::integral_constant<int, 4> four;
+    const std::integral_constant<int, 2> two;
     int r = 0;
     uint32_t lap = 0;
     for (int i = 0; i < n && ok; i++) {
       const int b = i & 1;
       const uint32_t before = (uint32_t)((i >> 1) - 1) & 1u;
       if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[b], before, wc, W_EMPTY, 47));
-      bool none[2], special[2];
-      const uint8_t* rec[2];
-      int left[2], r1 = r;
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[r1], lap, wc, W_FULL, 49));
-        if (!ok) break;
-        rec[h] = sm + M::RAW + r1 * REC;
-        uint8_t* kt = sm + M::K + b * M::KT + h * (kPage * 128);
-        left[h] = total - ((task.unit + i) * kManyStep + h * kPage);             // positions of the page that exist
-        none[h] = s_none[r1] != 0 || left[h] <= 0;
-        if (!none[h]) {
-          auto key = [&](int p, int w0, auto words) {            // words w0 .. of position p
-            constexpr int NWD = decltype(words)::value;
-            const uint8_t* blk = rec[h] + (p >> 4) * C::BLOCK;
-            uint32_t x[NWD];
-            if (NWD == 4) {
-              const uint4 w = *reinterpret_cast<const uint4*>(blk + C::k_word(p & 15, w0));
-              x[0] = w.x; x[1] = w.y; x[NWD - 2] = w.z; x[NWD - 1] = w.w;
-            } else {
-              const uint2 w = *reinterpret_cast<const uint2*>(blk + C::k_word(p & 15, w0));
-              x[0] = w.x; x[1] = w.y;
-            }
-            const uint32_t sz = *reinterpret_cast<const uint32_t*>(blk + C::KSZ + (p & 15) * 4);
-            const __nv_bfloat162 s = kv4_bf2(__byte_perm(sz, sz, 0x1010)), z = kv4_bf2(__byte_perm(sz, sz, 0x3232));
-            uint8_t* row = kt + (w0 >> 3) * (kManyStep * 128) + p * 128;
-#pragma unroll
-            for (int e = 0; e < NWD; e++)
-              *reinterpret_cast<uint4*>(row + ((((w0 + e) & 7) ^ (p & 7)) << 4)) =
-                  make_uint4(kv4_dequant2(x[e], s, z), kv4_dequant2(x[e] >> 4, s, z), kv4_dequant2(x[e] >> 8, s, z), kv4_dequant2(x[e] >> 12, s, z));
-          };
-          constexpr int QN = C::MAIN / 32, PT = 32 / QN, TURNS = kPage / PT;             // lanes of a position, positions of a turn
-          for (int j = (dw + 4 * h) % kManyDequant; j < TURNS; j += kManyDequant)
-            key(j * PT + lane / QN, 4 * (lane & (QN - 1)), std::integral_constant<int, 4>());
-          if (HD == 80 && dw >= 2 && dw < 4) key((dw - 2) * 32 + lane, 8, std::integral_constant<int, 2>());
-        }
-        if (++r1 == NR) { r1 = 0; lap ^= 1u; }
-      }
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[r], lap, wc, W_FULL, 49) && mbar_wait(&raw_full[r + 1], lap, wc, W_FULL, 49));
       if (!ok) break;
-      // V's NaN rows, and what lies behind the last position, become zeros: every row of P multiplies them
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        unsigned long long bad = 0;
-        if (!none[h]) {
-          const uint32_t a = *reinterpret_cast<const uint32_t*>(rec[h] + (lane >> 4) * C::BLOCK + C::VSZ + (lane & 15) * 4),
-                         c = *reinterpret_cast<const uint32_t*>(rec[h] + (2 + (lane >> 4)) * C::BLOCK + C::VSZ + (lane & 15) * 4);
-          bad = (unsigned long long)__ballot_sync(0xffffffffu, lane < left[h] && !(bflo(a) < INFINITY)) |
-                (unsigned long long)__ballot_sync(0xffffffffu, lane + 32 < left[h] && !(bflo(c) < INFINITY)) << 32;
-        }
-        special[h] = bad != 0 || left[h] < kPage;
-        if (dw == 0 && lane == 0) s_bad[2 * b + h] = bad;
+      const uint8_t *rec0 = sm + M::RAW + r * REC, *rec1 = rec0 + REC;
+      uint8_t *kt = sm + M::K + b * M::KT, *vt = sm + M::V + 2 * b * M::VT;
+      const int left0 = total - (task.unit + i) * kManyStep, left1 = left0 - kPage;                // positions of the pages that exist
+      const bool none0 = s_none[r] != 0, none1 = s_none[r + 1] != 0 || left1 <= 0;
+      // positions whose V is NaN: those, and what lies behind the last position, become zeros, as every row of P multiplies them
+      auto nan_of = [&](const uint8_t* rec, int left) {
+        const uint32_t a = *reinterpret_cast<const uint32_t*>(rec + (lane >> 4) * C::BLOCK + C::VSZ + (lane & 15) * 4),
+                       c = *reinterpret_cast<const uint32_t*>(rec + (2 + (lane >> 4)) * C::BLOCK + C::VSZ + (lane & 15) * 4);
+        return (unsigned long long)__ballot_sync(0xffffffffu, lane < left && !(bflo(a) < INFINITY)) |
+               (unsigned long long)__ballot_sync(0xffffffffu, lane + 32 < left && !(bflo(c) < INFINITY)) << 32;
+      };
+      const unsigned long long bad0 = none0 ? 0 : nan_of(rec0, left0), bad1 = none1 ? 0 : nan_of(rec1, left1);
+      const bool special = none0 || bad0 || bad1 || left1 < kPage;
+      if (dw == 0 && lane == 0) {
+        s_bad[2 * b] = bad0;
+        s_bad[2 * b + 1] = bad1;
+        s_gone[b] = (none0 ? 1 : 0) | (none1 ? 2 : 0);
       }
-      if (dw == 0 && lane == 0) s_gone[b] = (none[0] ? 1 : 0) | (none[1] ? 2 : 0);
+      if (!none0 && !none1) {
+#pragma unroll 1
+        for (int it = dw; it < 2 * KTURNS; it += kManyDequant) {
+          const int h = it / KTURNS, j = it % KTURNS;
+          key(h ? rec1 : rec0, kt + h * (kPage * 128), j * PT + lane / QN, 4 * (lane & (QN - 1)), four);
+        }
+        if (HD == 80 && dw >= 2) key(dw < 4 ? rec0 : rec1, kt + (dw < 4 ? 0 : kPage * 128), (dw & 1) * 32 + lane, 8, two);
+      } else {
+        for (int h = 0; h < 2; h++) {
+          if (h ? none1 : none0) continue;
+          for (int j = dw; j < KTURNS; j += kManyDequant) key(h ? rec1 : rec0, kt + h * (kPage * 128), j * PT + lane / QN, 4 * (lane & (QN - 1)), four);
+          if (HD == 80 && dw < 2) key(h ? rec1 : rec0, kt + h * (kPage * 128), dw * 32 + lane, 8, two);
+        }
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[b]);
       if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[b], before, wc, W_EMPTY, 48));
       if (!ok) break;
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        uint8_t* vt = sm + M::V + (2 * b + h) * M::VT;
-        auto value = [&](int c, int w, auto special_page) {      // dims 4w .. 4w+3 of positions 8c .. 8c+7
-          const uint8_t* blk = rec[h] + (c >> 1) * C::BLOCK;
-          uint32_t out[4][4];
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const int u = (c & 1) * 4 + k;
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(blk + C::v_word(u, w));
-            uint2 sz = *reinterpret_cast<const uint2*>(blk + C::VSZ + u * 8);
-            if (decltype(special_page)::value) {
-              if (8 * c + 2 * k >= left[h] || !(bflo(sz.x) < INFINITY)) sz.x = 0;
-              if (8 * c + 2 * k + 1 >= left[h] || !(bflo(sz.y) < INFINITY)) sz.y = 0;
-            }
-            const __nv_bfloat162 s = kv4_bf2(__byte_perm(sz.x, sz.y, 0x5410)), z = kv4_bf2(__byte_perm(sz.x, sz.y, 0x7632));
-#pragma unroll
-            for (int e = 0; e < 4; e++) out[e][k] = kv4_dequant2(x >> (4 * e), s, z);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int d = 4 * w + e;
-            *reinterpret_cast<uint4*>(vt + d * 128 + ((c ^ (d & 7)) << 4)) = make_uint4(out[e][0], out[e][1], out[e][2], out[e][3]);
-          }
-        };
-        if (none[h]) {
-          for (int k = tid - 256; k < M::VT / 16; k += kManyDequant * 32) *reinterpret_cast<uint4*>(vt + k * 16) = make_uint4(0, 0, 0, 0);
-        } else {
-          // a phase of eight lanes stores to eight chunks; four chunks' lanes read words of different bank groups
-          const int ci = (lane >> 1) & 3, wi = (lane & 1) | (lane >> 3) << 1;
-          constexpr int NG = C::MAIN / 32;                       // groups of eight words
-          auto turns = [&](auto special_page) {
-            for (int j = (dw + 4 * h) % kManyDequant; j < 2 * NG; j += kManyDequant) value(4 * (j & 1) + ci, 8 * (((j >> 1) + ci) & (NG - 1)) + wi, special_page);
-            if (HD == 80 && dw == (h ? 5 : 4)) value((lane >> 1) & 7, 16 + ((lane & 1) | (lane >> 4) << 1), special_page);
-          };
-          if (special[h]) turns(std::true_type());
-          else turns(std::false_type());
+      if (!special) {
+#pragma unroll 1
+        for (int it = (dw + 4) % kManyDequant; it < 2 * VTURNS; it += kManyDequant) {                // who had one K turn less begins
+          const int h = it / VTURNS, j = it % VTURNS;
+          value(h ? rec1 : rec0, vt + h * M::VT, chunk_of(j), word_of(j), 0, std::false_type());
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&raw_empty[r]);
-        if (++r == NR) r = 0;
+        if (HD == 80 && dw < 2) value(dw ? rec1 : rec0, vt + dw * M::VT, (lane >> 1) & 7, 16 + ((lane & 1) | (lane >> 4) << 1), 0, std::false_type());
+      } else {
+        for (int h = 0; h < 2; h++) {
+          const uint8_t* rec = h ? rec1 : rec0;
+          if (h ? none1 : none0) {
+            for (int k = tid - 256; k < M::VT / 16; k += kManyDequant * 32) *reinterpret_cast<uint4*>(vt + h * M::VT + k * 16) = make_uint4(0, 0, 0, 0);
+            continue;
+          }
+          const int left = h ? left1 : left0;
+          for (int j = dw; j < VTURNS; j += kManyDequant) value(rec, vt + h * M::VT, chunk_of(j), word_of(j), left, std::true_type());
+          if (HD == 80 && dw == 5) value(rec, vt + h * M::VT, (lane >> 1) & 7, 16 + ((lane & 1) | (lane >> 4) << 1), left, std::true_type());
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[b]);
+      if (lane == 0) { mbar_arrive(&raw_empty[r]); mbar_arrive(&raw_empty[r + 1]); mbar_arrive(&v_full[b]); }
+      r += 2;
+      if (r == NR) { r = 0; lap ^= 1u; }
     }
   }
   } else {
