@@ -24,7 +24,7 @@ struct Kv4Many {
   static constexpr int QT = NB * 128 * 128, KT = NB * kManyStep * 128, VT = HD * 128;      // bytes: Q tile, K step, V page
   static constexpr int NR = 4;                                              // pages: two being dequantised, two on their way
   static constexpr int Q = 0, K = Q + 2 * QT, V = K + 2 * KT, RAW = V + 4 * VT, BAR = RAW + NR * REC;
-  static constexpr int BARS = 2 * NR + 15, TOTAL = BAR + BARS * 8 + 4 * 8 + (2 + 5 + NR + 2) * 4;       // barriers, then what stands behind them in the kernel
+  static constexpr int BARS = 2 * NR + 17, TOTAL = BAR + BARS * 8 + 4 * 8 + (2 + 5 + NR + 2) * 4;       // barriers, then what stands behind them in the kernel
   static constexpr int T_S = 0, T_O = 256, TCOLS = 512;                     // tensor memory columns: two S / P, two O
   static_assert(TOTAL <= 227 * 1024 && T_O + 2 * HD <= TCOLS && QT % 1024 == 0 && VT % 1024 == 0 && RAW % 16 == 0 && REC % 16 == 0, "plan");
 };
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
   uint8_t* const sm = many_sm;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + M::BAR);
   uint64_t *raw_full = bars, *raw_empty = raw_full + NR, *k_full = raw_empty + NR, *k_empty = k_full + 2, *v_full = k_empty + 2, *v_empty = v_full + 2,
-           *s_full = v_empty + 2, *p_full = s_full + 2, *pv_done = p_full + 2, *q_full = pv_done + 2;
+           *s_full = v_empty + 2, *p_full = s_full + 2, *pv_done = p_full + 4, *q_full = pv_done + 2;
   unsigned long long* s_bad = reinterpret_cast<unsigned long long*>(bars + M::BARS);   // [2 steps][2 pages] positions whose V is NaN
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_bad + 4);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
     for (int i = 0; i < NR; i++) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], kManyDequant); }
     for (int i = 0; i < 2; i++) {
       mbar_init(&k_full[i], kManyDequant); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], kManyDequant); mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&pv_done[i], 1);
+      mbar_init(&s_full[i], 1); mbar_init(&p_full[2 * i], 4); mbar_init(&p_full[2 * i + 1], 4); mbar_init(&pv_done[i], 1);
     }
     mbar_init(q_full, 4 * tiles);
     *s_abort = 0;
@@ -168,20 +168,22 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       __syncwarp();
       if (lane == 0) s_issued[1 + t] = i + 1;
     };
-    auto pv = [&](auto tile, int i) {
-      constexpr int t = decltype(tile)::value;
+    auto pv = [&](auto tile, auto part, int i) {                 // of the step's first or second page
+      constexpr int t = decltype(tile)::value, h = decltype(part)::value;
       if (elect_one()) {
-        const uint64_t vb = v0 + (uint64_t)((i & 1) * (M::VT >> 3));
+        const uint64_t vb = v0 + (uint64_t)((i & 1) * (M::VT >> 3) + h * (M::VT >> 4));
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
+        for (int k = 0; k < 4; k++) {
           constexpr uint32_t id = idesc | ((uint32_t)(HD >> 3) << 17);
-          tc_mma_ts(tmem + M::T_O + t * HD, tmem + M::T_S + t * 128 + k * 8, vb + (uint64_t)(((k >> 2) * M::VT + (k & 3) * 32) >> 4), id, i || k ? 1u : 0u);
+          tc_mma_ts(tmem + M::T_O + t * HD, tmem + M::T_S + t * 128 + (4 * h + k) * 8, vb + (uint64_t)((k * 32) >> 4), id, i || h || k ? 1u : 0u);
         }
-        tc_commit(&pv_done[t]);
-        if (t == tiles - 1) tc_commit(&v_empty[i & 1]);
+        if (h) {
+          tc_commit(&pv_done[t]);
+          if (t == tiles - 1) tc_commit(&v_empty[i & 1]);
+        }
       }
       __syncwarp();
-      if (lane == 0) s_issued[3 + t] = i + 1;
+      if (h && lane == 0) s_issued[3 + t] = i + 1;
     };
     auto wait = [&](uint64_t* bar, int i, int where) {           // phase i of a barrier
       ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, (uint32_t)i & 1u, wc, W_FULL, where));
@@ -196,8 +198,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
     }
     auto turn = [&](auto tile, int i) {
       constexpr int t = decltype(tile)::value;
-      if (!wait(&p_full[t], i, 43) || (t == 0 && !wait(&v_full[i & 1], i >> 1, 44))) return;
-      pv(tile, i);
+      if (!wait(&p_full[2 * t], i, 43) || (t == 0 && !wait(&v_full[i & 1], i >> 1, 44))) return;
+      pv(tile, first, i);
+      if (!wait(&p_full[2 * t + 1], i, 43)) return;
+      pv(tile, second, i);
       if (i + 1 == n || (t == 0 && !wait(&k_full[(i + 1) & 1], (i + 1) >> 1, 45)) || !wait(&pv_done[t], i, 46)) return;
       qk(tile, i + 1);
     };
@@ -426,15 +430,17 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
           asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[e]) : "f"(d), "f"(a));
         }
         tc_st16(ts + c * 16, o);
+        if (c & 1) {                                             // a page's half of P is there
+          tc_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * t + (c >> 1)]);
+        }
       }
       {
         const float2 y = f32x2_of(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])));
         l += y.x + y.y;
       }
-      tc_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[t]);
     }
     if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (uint32_t)(n - 1) & 1u, wc, W_FULL, 52));
     tc_fence_after();
