@@ -22,9 +22,10 @@ template <int HD>
 struct Kv4Many {
   static constexpr int REC = Kv4<HD>::REC, NB = HD == 64 ? 1 : 2;           // blocks of 64 dims of a K-major tile
   static constexpr int QT = NB * 128 * 128, KT = NB * kManyStep * 128, VT = HD * 128;      // bytes: Q tile, K step, V page
+  static constexpr int ND = 4;                                              // steps whose notes are kept: softmax may be at i when step i + 2 is dequantised
   static constexpr int NR = 4;                                              // pages: two being dequantised, two on their way
   static constexpr int Q = 0, K = Q + 2 * QT, V = K + 2 * KT, RAW = V + 4 * VT, BAR = RAW + NR * REC;
-  static constexpr int BARS = 2 * NR + 17, TOTAL = BAR + BARS * 8 + 4 * 8 + (2 + 5 + NR + 2) * 4;       // barriers, then what stands behind them in the kernel
+  static constexpr int BARS = 2 * NR + 17, TOTAL = BAR + BARS * 8 + 2 * ND * 8 + (2 + 5 + NR + ND) * 4;       // barriers, then what stands behind them in the kernel
   static constexpr int T_S = 0, T_O = 256, TCOLS = 512;                     // tensor memory columns: two S / P, two O
   static_assert(TOTAL <= 227 * 1024 && T_O + 2 * HD <= TCOLS && QT % 1024 == 0 && VT % 1024 == 0 && RAW % 16 == 0 && REC % 16 == 0, "plan");
 };
@@ -85,12 +86,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + M::BAR);
   uint64_t *raw_full = bars, *raw_empty = raw_full + NR, *k_full = raw_empty + NR, *k_empty = k_full + 2, *v_full = k_empty + 2, *v_empty = v_full + 2,
            *s_full = v_empty + 2, *p_full = s_full + 2, *pv_done = p_full + 4, *q_full = pv_done + 2;
-  unsigned long long* s_bad = reinterpret_cast<unsigned long long*>(bars + M::BARS);   // [2 steps][2 pages] positions whose V is NaN
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_bad + 4);
+  unsigned long long* s_bad = reinterpret_cast<unsigned long long*>(bars + M::BARS);   // [ND steps][2 pages] positions whose V is NaN
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_bad + 2 * M::ND);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   volatile int* s_issued = s_abort + 1;                          // [5] pages, QK of tiles 0 and 1, PV of tiles 0 and 1
   volatile int* s_none = s_issued + 5;                           // [NR] the page does not exist
-  volatile int* s_gone = s_none + NR;                            // [2 steps] bit p: page p of the step does not exist
+  volatile int* s_gone = s_none + NR;                            // [ND steps] bit p: page p of the step does not exist
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Kv4Seqs& S = P.S;
   pdl_begin(true);
@@ -284,9 +285,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       const unsigned long long bad0 = none0 ? 0 : nan_of(rec0, left0), bad1 = none1 ? 0 : nan_of(rec1, left1);
       const bool special = none0 || bad0 || bad1 || left1 < kPage;
       if (dw == 0 && lane == 0) {
-        s_bad[2 * b] = bad0;
-        s_bad[2 * b + 1] = bad1;
-        s_gone[b] = (none0 ? 1 : 0) | (none1 ? 2 : 0);
+        // Their place was step i - 4's: the softmax of that one has read it, as PV of step i - 3 has ended (the wait for V's place of the step before)
+        const int note = i & (M::ND - 1);
+        s_bad[2 * note] = bad0;
+        s_bad[2 * note + 1] = bad1;
+        s_gone[note] = (none0 ? 1 : 0) | (none1 ? 2 : 0);
       }
       if (!none0 && !none1) {
 #pragma unroll 1
@@ -366,8 +369,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       uint32_t v[4][32];                                         // the row's scores, then its probabilities, stay in registers
 #pragma unroll
       for (int c = 0; c < 4; c++) tc_ld32(ts + c * 32, v[c]);
-      const int p0 = (task.unit + i) * kManyStep, gone = s_gone[i & 1];
-      const unsigned long long bad0 = s_bad[2 * (i & 1)], bad1 = s_bad[2 * (i & 1) + 1];
+      const int p0 = (task.unit + i) * kManyStep, note = i & (M::ND - 1), gone = s_gone[note];
+      const unsigned long long bad0 = s_bad[2 * note], bad1 = s_bad[2 * note + 1];
       tc_ld_wait();
       if (p0 + kManyStep > (mask ? seq.cached : min(total, seq.cached + m_first + 1)) || gone || (bad0 | bad1)) {
         // what is not seen becomes -inf

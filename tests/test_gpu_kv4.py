@@ -285,6 +285,20 @@ def test_values_whose_scales_span_many_powers_of_two():
         assert out.isfinite().all()
 
 
+@pytest.mark.parametrize("hd", [64, 80, 128])
+def test_a_none_of_a_later_step_stays_there(hd):
+    """Steps of 128 positions follow one another while the softmax of earlier ones runs: a value that is none in the third is not held against the first."""
+    nh, nkv, cached, new = 16, 4, 256, 64
+    c, K, V, q, _ = filled([cached], [new], nh, nkv, hd, seed=5)
+    bad = torch.full((1, nkv, hd), math.nan, dtype=torch.bfloat16, device=DEV)
+    c.append(0, rows(21, 1, nkv, hd), bad, cached + 40)
+    outs = [c.attend(0, q, cached) for _ in range(40)]
+    c.check()
+    for out in outs:
+        assert out[:40].isfinite().all() and out[40:].isnan().all()
+        assert torch.equal(out[:40], outs[0][:40])
+
+
 @pytest.mark.parametrize("new", [1, 40])
 @pytest.mark.parametrize("at", [0, 40, 199])
 def test_large_values_of_small_weight_leave_the_others_as_they_are(new, at):
