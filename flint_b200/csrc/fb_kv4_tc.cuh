@@ -4,9 +4,11 @@
 // 128 (two pages). Per step and tile: S[128 rows][128 positions] = Q K^T into tensor memory, softmax by a warpgroup (a thread a row: no shuffles), P as bf16 back
 // into tensor memory over S, O[128][HD] += P V. Tensor pipe and exponentials (16 a clock and SM) need the same 1024 clocks a tile and step at heads of 128, so the two
 // tiles take turns: one multiplies while the other exponentiates. Keys and values are dequantised once for both tiles by eight warps into the K-major
-// 128-byte-swizzle layout that the MMA reads, K as [position][dim], V as [dim][position]: (nib - 8) s + z in bf16, rounded once, the precision of a bf16 cache (half
-// a step is 2^-8), and with bf16's range, so that rows of any size stand side by side. (Operands nib - 8, with s and z in the softmax as kv4_attn_few has
-// them, would be exact, but cost the softmax, which is what bounds this kernel, twice its instructions.) P is bf16 as well, sums and maxima are fp32.
+// 128-byte-swizzle layout that the MMA reads, K as [position][dim], V as [dim][position], each number (nib - 8) s + z rounded once. (Operands nib - 8, with s and z in the
+// softmax as kv4_attn_few has them, would be exact, but cost the softmax, which is what bounds this kernel, twice its instructions.) All operands are fp16, half a step
+// 2^-11: K times a power of two per step (2^-25 of the largest key of its 128 positions at the smallest), Q times one per row, P times 2^7, V as it is. A page
+// whose rows of V do not all lie within fp16's range has its V and P in bf16, half a step 2^-8: there rows of any size stand side by side, whatever their
+// weight. (With bf16 operands throughout, outputs were off by 0.0044 of their 2-norm; now 0.0017, the rounding of the output itself.) Sums and maxima are fp32.
 // The maximum is moved, and O rescaled, only when a score exceeds it by more than 2^8.
 // Warps: 0..3 and 4..7 softmax of tiles 0 and 1 (and Q in, O out), 8..13 dequantise, 14 brings pages (one bulk copy each), 15 issues MMAs.
 #pragma once
@@ -16,6 +18,7 @@
 namespace fb {
 
 constexpr int kManyThreads = 16 * 32, kManyRows = 256, kManyStep = 128;
+constexpr float kManyLift = 7.f;                   // probabilities are 2^7 times what they are, 2^15 at most: in fp16 they lose nothing down to 2^-21
 constexpr int kManyDequant = 6;                    // warps that dequantise
 
 template <int HD>
@@ -25,7 +28,7 @@ struct Kv4Many {
   static constexpr int ND = 4;                                              // steps whose notes are kept: softmax may be at i when step i + 2 is dequantised
   static constexpr int NR = 4;                                              // pages: two being dequantised, two on their way
   static constexpr int Q = 0, K = Q + 2 * QT, V = K + 2 * KT, RAW = V + 4 * VT, BAR = RAW + NR * REC;
-  static constexpr int BARS = 2 * NR + 17, TOTAL = BAR + BARS * 8 + 2 * ND * 8 + (2 + 5 + NR + ND) * 4;       // barriers, then what stands behind them in the kernel
+  static constexpr int BARS = 2 * NR + 17, TOTAL = BAR + BARS * 8 + 2 * ND * 8 + (2 + 5 + NR + 2 * ND) * 4;       // barriers, then what stands behind them in the kernel
   static constexpr int T_S = 0, T_O = 256, TCOLS = 512;                     // tensor memory columns: two S / P, two O
   static_assert(TOTAL <= 227 * 1024 && T_O + 2 * HD <= TCOLS && QT % 1024 == 0 && VT % 1024 == 0 && RAW % 16 == 0 && REC % 16 == 0, "plan");
 };
@@ -34,6 +37,16 @@ __device__ __forceinline__ uint32_t kv4_dequant2(uint32_t w, __nv_bfloat162 s, _
   const uint32_t x = (w & 0x000F000Fu) | 0x43004300u;            // 128 + nib
   const uint32_t k136 = 0x43084308u;
   const __nv_bfloat162 r = __hfma2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&k136)), s, z);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// ... fp16, nibbles in bits 0..3 and 16..19, or 4..7 and 20..23 (nib - 8 is exact, one rounding follows)
+__device__ __forceinline__ __half2 kv4_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+__device__ __forceinline__ uint32_t kv4_half_lo(uint32_t w, __half2 s, __half2 z) {
+  const __half2 r = __hfma2(__hsub2(kv4_h2((w & 0x000F000Fu) | 0x64006400u), kv4_h2(0x64086408u)), s, z);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t kv4_half_hi(uint32_t w, __half2 s, __half2 z) {
+  const __half2 r = __hfma2(__hfma2(kv4_h2((w & 0x00F000F0u) | 0x64006400u), kv4_h2(0x2C002C00u), kv4_h2(0xD480D480u)), s, z);
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ __nv_bfloat162 kv4_bf2(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
@@ -91,7 +104,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   volatile int* s_issued = s_abort + 1;                          // [5] pages, QK of tiles 0 and 1, PV of tiles 0 and 1
   volatile int* s_none = s_issued + 5;                           // [NR] the page does not exist
-  volatile int* s_gone = s_none + NR;                            // [ND steps] bit p: page p of the step does not exist
+  volatile int* s_gone = s_none + NR;                            // [ND steps] bit p: page p of the step does not exist, bit 2 + p: it is wide
+  volatile float* s_kscale = reinterpret_cast<volatile float*>(s_gone + M::ND);  // [ND steps] inverse of the power of two of the keys
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Kv4Seqs& S = P.S;
   pdl_begin(true);
@@ -151,7 +165,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
     if (lane == 0) s_issued[0] = issued;
   } else if (warp == 15) {
     // ---------------- MMA issue: per tile PV of a step, then QK of the next one once PV has read P, which lies over S
-    constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);               // bf16 x bf16 -> fp32, 128 rows
+    constexpr uint32_t idesc = (1u << 4) | ((128u >> 4) << 24), bf16 = (1u << 7) | (1u << 10);        // fp16 x fp16 (or bf16 x bf16) -> fp32, 128 rows
     const uint64_t q0 = tc_desc(smem_u32(sm + M::Q)), k0 = tc_desc(smem_u32(sm + M::K)), v0 = tc_desc(smem_u32(sm + M::V));
     auto qk = [&](auto tile, int i) {
       constexpr int t = decltype(tile)::value;
@@ -171,11 +185,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
     };
     auto pv = [&](auto tile, auto part, int i) {                 // of the step's first or second page
       constexpr int t = decltype(tile)::value, h = decltype(part)::value;
+      const uint32_t id = idesc | (s_gone[i & (M::ND - 1)] >> h & 4 ? bf16 : 0u) | ((uint32_t)(HD >> 3) << 17);
       if (elect_one()) {
         const uint64_t vb = v0 + (uint64_t)((i & 1) * (M::VT >> 3) + h * (M::VT >> 4));
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          constexpr uint32_t id = idesc | ((uint32_t)(HD >> 3) << 17);
           tc_mma_ts(tmem + M::T_O + t * HD, tmem + M::T_S + t * 128 + (4 * h + k) * 8, vb + (uint64_t)((k * 32) >> 4), id, i || h || k ? 1u : 0u);
         }
         if (h) {
@@ -216,6 +230,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
     // The turns of both pages are dealt out to the warps together. (Unrolled, they do not fit 80 registers: 160 us of 1000 tokens behind 7011 became 204.)
     const int dw = warp - 8;
     constexpr int QN = C::MAIN / 32, PT = 32 / QN, KTURNS = kPage / PT, VTURNS = C::MAIN / 16;       // lanes of a position, positions of a turn, turns of a page
+    float kf = 1.f;                                              // the step's power of two of the keys
     auto key = [&](const uint8_t* rec, uint8_t* kt, int p, int w0, auto words) {           // words w0 .. of position p
       constexpr int NWD = decltype(words)::value;
       const uint8_t* blk = rec + (p >> 4) * C::BLOCK;
@@ -228,14 +243,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
         x[0] = w.x; x[1] = w.y;
       }
       const uint32_t sz = *reinterpret_cast<const uint32_t*>(blk + C::KSZ + (p & 15) * 4);
-      const __nv_bfloat162 s = kv4_bf2(__byte_perm(sz, sz, 0x1010)), z = kv4_bf2(__byte_perm(sz, sz, 0x3232));
+      const uint32_t f = cvt_f16x2(bflo(sz) * kf, bfhi(sz) * kf);
+      const __half2 s = kv4_h2(__byte_perm(f, f, 0x1010)), z = kv4_h2(__byte_perm(f, f, 0x3232));
       uint8_t* row = kt + (w0 >> 3) * (kManyStep * 128) + p * 128;
 #pragma unroll
       for (int e = 0; e < NWD; e++)
         *reinterpret_cast<uint4*>(row + ((((w0 + e) & 7) ^ (p & 7)) << 4)) =
-            make_uint4(kv4_dequant2(x[e], s, z), kv4_dequant2(x[e] >> 4, s, z), kv4_dequant2(x[e] >> 8, s, z), kv4_dequant2(x[e] >> 12, s, z));
+            make_uint4(kv4_half_lo(x[e], s, z), kv4_half_hi(x[e], s, z), kv4_half_lo(x[e] >> 8, s, z), kv4_half_hi(x[e] >> 8, s, z));
     };
-    auto value = [&](const uint8_t* rec, uint8_t* vt, int c, int w, int left, auto special) {        // dims 4w .. 4w+3 of positions 8c .. 8c+7
+    auto value = [&](const uint8_t* rec, uint8_t* vt, int c, int w, int left, bool wide, auto special) {        // dims 4w .. 4w+3 of positions 8c .. 8c+7
       const uint8_t* blk = rec + (c >> 1) * C::BLOCK;
       uint32_t out[4][4];
 #pragma unroll
@@ -247,9 +263,17 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
           if (8 * c + 2 * k >= left || !(bflo(sz.x) < INFINITY)) sz.x = 0;
           if (8 * c + 2 * k + 1 >= left || !(bflo(sz.y) < INFINITY)) sz.y = 0;
         }
-        const __nv_bfloat162 s = kv4_bf2(__byte_perm(sz.x, sz.y, 0x5410)), z = kv4_bf2(__byte_perm(sz.x, sz.y, 0x7632));
+        if (decltype(special)::value && wide) {
+          const __nv_bfloat162 s = kv4_bf2(__byte_perm(sz.x, sz.y, 0x5410)), z = kv4_bf2(__byte_perm(sz.x, sz.y, 0x7632));
 #pragma unroll
-        for (int e = 0; e < 4; e++) out[e][k] = kv4_dequant2(x >> (4 * e), s, z);
+          for (int e = 0; e < 4; e++) out[e][k] = kv4_dequant2(x >> (4 * e), s, z);
+        } else {
+          const __half2 s = kv4_h2(cvt_f16x2(bflo(sz.x), bflo(sz.y))), z = kv4_h2(cvt_f16x2(bfhi(sz.x), bfhi(sz.y)));
+          out[0][k] = kv4_half_lo(x, s, z);
+          out[1][k] = kv4_half_hi(x, s, z);
+          out[2][k] = kv4_half_lo(x >> 8, s, z);
+          out[3][k] = kv4_half_hi(x >> 8, s, z);
+        }
       }
 #pragma unroll
       for (int e = 0; e < 4; e++) {
@@ -275,21 +299,35 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       uint8_t *kt = sm + M::K + b * M::KT, *vt = sm + M::V + 2 * b * M::VT;
       const int left0 = total - (task.unit + i) * kManyStep, left1 = left0 - kPage;                // positions of the pages that exist
       const bool none0 = s_none[r] != 0, none1 = s_none[r + 1] != 0 || left1 <= 0;
-      // positions whose V is NaN: those, and what lies behind the last position, become zeros, as every row of P multiplies them
-      auto nan_of = [&](const uint8_t* rec, int left) {
-        const uint32_t a = *reinterpret_cast<const uint32_t*>(rec + (lane >> 4) * C::BLOCK + C::VSZ + (lane & 15) * 4),
-                       c = *reinterpret_cast<const uint32_t*>(rec + (2 + (lane >> 4)) * C::BLOCK + C::VSZ + (lane & 15) * 4);
-        return (unsigned long long)__ballot_sync(0xffffffffu, lane < left && !(bflo(a) < INFINITY)) |
-               (unsigned long long)__ballot_sync(0xffffffffu, lane + 32 < left && !(bflo(c) < INFINITY)) << 32;
+      // Positions whose V is NaN: those, and what lies behind the last position, become zeros, as every row of P multiplies them. A page whose rows of V
+      // have bounds 8 |s| + |z| (its largest value that there can be) beyond [2^-10, 2^15) is `wide`; kmost: the largest bound of a key.
+      uint32_t kmost = 0;
+      bool wide0 = false, wide1 = false;
+      auto look = [&](const uint8_t* rec, int left, bool& wide) {
+        uint32_t bad[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const uint8_t* at = rec + (2 * k + (lane >> 4)) * C::BLOCK + (lane & 15) * 4;
+          const uint32_t a = *reinterpret_cast<const uint32_t*>(at + C::KSZ), c = *reinterpret_cast<const uint32_t*>(at + C::VSZ);
+          const bool in = 32 * k + lane < left, num = bflo(c) < INFINITY;
+          const float kb = fmaf(8.f, fabsf(bflo(a)), fabsf(bfhi(a))), vb = fmaf(8.f, fabsf(bflo(c)), fabsf(bfhi(c)));
+          if (in && kb < INFINITY) kmost = max(kmost, __float_as_uint(kb));
+          bad[k] = __ballot_sync(0xffffffffu, in && !num);
+          wide |= __any_sync(0xffffffffu, in && num && vb != 0.f && !(vb >= 0x1p-10f && vb < 0x1p15f)) != 0;
+        }
+        return (unsigned long long)bad[0] | (unsigned long long)bad[1] << 32;
       };
-      const unsigned long long bad0 = none0 ? 0 : nan_of(rec0, left0), bad1 = none1 ? 0 : nan_of(rec1, left1);
-      const bool special = none0 || bad0 || bad1 || left1 < kPage;
+      const unsigned long long bad0 = none0 ? 0 : look(rec0, left0, wide0), bad1 = none1 ? 0 : look(rec1, left1, wide1);
+      const float2 kp = pow2_for(__uint_as_float(__reduce_max_sync(0xffffffffu, kmost)));          // the largest into [2^14, 2^15)
+      kf = kp.x;
+      const bool special = none0 || bad0 || bad1 || left1 < kPage || wide0 || wide1;
       if (dw == 0 && lane == 0) {
         // Their place was step i - 4's: the softmax of that one has read it, as PV of step i - 3 has ended (the wait for V's place of the step before)
         const int note = i & (M::ND - 1);
         s_bad[2 * note] = bad0;
         s_bad[2 * note + 1] = bad1;
-        s_gone[note] = (none0 ? 1 : 0) | (none1 ? 2 : 0);
+        s_gone[note] = (none0 ? 1 : 0) | (none1 ? 2 : 0) | (wide0 ? 4 : 0) | (wide1 ? 8 : 0);
+        s_kscale[note] = kp.y;
       }
       if (!none0 && !none1) {
 #pragma unroll 1
@@ -314,9 +352,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
 #pragma unroll 1
         for (int it = (dw + 4) % kManyDequant; it < 2 * VTURNS; it += kManyDequant) {                // who had one K turn less begins
           const int h = it / VTURNS, j = it % VTURNS;
-          value(h ? rec1 : rec0, vt + h * M::VT, chunk_of(j), word_of(j), 0, std::false_type());
+          value(h ? rec1 : rec0, vt + h * M::VT, chunk_of(j), word_of(j), 0, false, std::false_type());
         }
-        if (HD == 80 && dw < 2) value(dw ? rec1 : rec0, vt + dw * M::VT, (lane >> 1) & 7, 16 + ((lane & 1) | (lane >> 4) << 1), 0, std::false_type());
+        if (HD == 80 && dw < 2) value(dw ? rec1 : rec0, vt + dw * M::VT, (lane >> 1) & 7, 16 + ((lane & 1) | (lane >> 4) << 1), 0, false, std::false_type());
       } else {
         for (int h = 0; h < 2; h++) {
           const uint8_t* rec = h ? rec1 : rec0;
@@ -325,8 +363,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
             continue;
           }
           const int left = h ? left1 : left0;
-          for (int j = dw; j < VTURNS; j += kManyDequant) value(rec, vt + h * M::VT, chunk_of(j), word_of(j), left, std::true_type());
-          if (HD == 80 && dw == 5) value(rec, vt + h * M::VT, (lane >> 1) & 7, 16 + ((lane & 1) | (lane >> 4) << 1), left, std::true_type());
+          for (int j = dw; j < VTURNS; j += kManyDequant) value(rec, vt + h * M::VT, chunk_of(j), word_of(j), left, h ? wide1 : wide0, std::true_type());
+          if (HD == 80 && dw == 5) value(rec, vt + h * M::VT, (lane >> 1) & 7, 16 + ((lane & 1) | (lane >> 4) << 1), left, h ? wide1 : wide0, std::true_type());
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -344,21 +382,31 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = tl + M::T_S + t * 128, to = tl + M::T_O + t * HD;
     const bool live = lr < rows;
     const int gr = task.r0 + min(lr, rows - 1), mq = gr / R, head = kvh * R + gr % R;
-    {                                                            // Q: the row into the swizzled tile; a negative scale is a negative Q
+    float cs = fabsf(P.scale);
+    {                                                            // Q: the row, as fp16 times a power of two, into the swizzled tile; a negative scale is a negative Q
       const uint16_t* src = P.q + (size_t)(seq.first + mq) * P.q_ld + (size_t)head * HD;
       const uint32_t flip = P.scale < 0.f ? 0x80008000u : 0u;
       uint8_t* qt = sm + M::Q + t * M::QT + row * 128;
+      uint32_t w[HD / 2], most = 0;
 #pragma unroll
       for (int c = 0; c < HD / 8; c++) {
-        uint4 v = live ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
-        v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-        *reinterpret_cast<uint4*>(qt + (c >> 3) * (128 * 128) + (((c & 7) ^ (row & 7)) << 4)) = v;
+        const uint4 v = live ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+        w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
+      }
+#pragma unroll
+      for (int k = 0; k < HD / 2; k++) most = __vmaxu2(most, w[k] & 0x7fff7fffu);
+      const float2 f = pow2_for(__uint_as_float(max(most & 0xffffu, most >> 16) << 16));
+      cs *= f.y;
+#pragma unroll
+      for (int c = 0; c < HD / 8; c++) {
+        auto half2_of = [&](uint32_t v) { return cvt_f16x2(bflo(v ^ flip) * f.x, bfhi(v ^ flip) * f.x); };
+        *reinterpret_cast<uint4*>(qt + (c >> 3) * (128 * 128) + (((c & 7) ^ (row & 7)) << 4)) =
+            make_uint4(half2_of(w[4 * c]), half2_of(w[4 * c + 1]), half2_of(w[4 * c + 2]), half2_of(w[4 * c + 3]));
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
-    const float cs = fmaxf(fabsf(P.scale), 1e-30f);              // not zero: a score that is not seen stays -inf
     const uint8_t* mask = P.amask ? P.amask + (size_t)(seq.first + mq) * P.mask_ld : nullptr;
     const int m_first = (task.r0 + min(t * 128 + (warp & 3) * 32, rows - 1)) / R;          // the warp's first token: what it sees, all rows see
     float m = -1e30f, l = 0.f;
@@ -370,9 +418,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
 #pragma unroll
       for (int c = 0; c < 4; c++) tc_ld32(ts + c * 32, v[c]);
       const int p0 = (task.unit + i) * kManyStep, note = i & (M::ND - 1), gone = s_gone[note];
+      const float c2 = fmaxf(cs * s_kscale[note], 1.2e-38f);     // not zero: a score that is not seen stays -inf
       const unsigned long long bad0 = s_bad[2 * note], bad1 = s_bad[2 * note + 1];
       tc_ld_wait();
-      if (p0 + kManyStep > (mask ? seq.cached : min(total, seq.cached + m_first + 1)) || gone || (bad0 | bad1)) {
+      if (p0 + kManyStep > (mask ? seq.cached : min(total, seq.cached + m_first + 1)) || (gone & 3) || (bad0 | bad1)) {
         // what is not seen becomes -inf
         uint32_t vis[4];
 #pragma unroll
@@ -400,7 +449,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       for (int c = 0; c < 4; c++)
 #pragma unroll
         for (int e = 0; e < 32; e += 2) mx[(e >> 1) & 7] = max3(mx[(e >> 1) & 7], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
-      const float top = fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[4]), max3(mx[5], mx[6], mx[7])) * cs;
+      const float top = fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[4]), max3(mx[5], mx[6], mx[7])) * c2;
       if (__any_sync(0xffffffffu, top > m + 8.f)) {
         const float mn = fmaxf(m, top), corr = ex2(m - mn);
         if (i > 0) {                                             // O as the steps before left it
@@ -420,25 +469,33 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
         m = mn;
         l *= corr;
       }
-      const uint64_t cs2 = f32x2(cs, cs), m2 = f32x2(-m, -m);
+      const uint64_t cs2 = f32x2(c2, c2), m2 = f32x2(kManyLift - m, kManyLift - m);
       uint64_t sum[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
+      auto powers = [&](int c, auto wide) {                      // P of 32 positions
         uint32_t o[16];
 #pragma unroll
         for (int e = 0; e < 16; e++) {
           const float2 y = f32x2_of(fma_f32x2(f32x2(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), cs2, m2));
           const float a = ex2(y.x), d = ex2(y.y);
           sum[e & 3] = add_f32x2(sum[e & 3], f32x2(a, d));
-          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[e]) : "f"(d), "f"(a));
+          if (decltype(wide)::value) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[e]) : "f"(d), "f"(a));
+          else o[e] = cvt_f16x2(a, d);
         }
         tc_st16(ts + c * 16, o);
-        if (c & 1) {                                             // a page's half of P is there
-          tc_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[2 * t + (c >> 1)]);
+      };
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        if (gone >> h & 4) {
+          powers(2 * h, std::true_type());
+          powers(2 * h + 1, std::true_type());
+        } else {
+          powers(2 * h, std::false_type());
+          powers(2 * h + 1, std::false_type());
         }
+        tc_st_wait();                                            // a page's half of P is there
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * t + h]);
       }
       {
         const float2 y = f32x2_of(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])));
@@ -476,7 +533,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
         }
         __syncwarp();
       }
-      if (w && live) *reinterpret_cast<float2*>(w + HD) = make_float2(m, l);
+      if (w && live) *reinterpret_cast<float2*>(w + HD) = make_float2(m - kManyLift, l);
     }
   }
   }

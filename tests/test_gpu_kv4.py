@@ -152,16 +152,18 @@ def test_ragged_sequences_depths_strides_and_tokens_behind_the_last_sequence():
 
 
 # ---------------------------------------------------------------------------------------------------------------- attention
-def check_attention(out, q, K, V, cached, scale, amask=None, many=False):
+def check_attention(out, q, K, V, cached, scale, amask=None, many=False, wide=False):
     """K, V: what the cache stands for. The kernels' own roundings (each at most half a step): the output to bf16 (2^-8 of the value); sums in 32 bits. Up to 64 query rows
     a kv head: probabilities to fp16 (2^-11 of each, 2^-25 of the largest one for those below 2^-14 of it), keys and values as they are. More rows:
-    probabilities, keys and values to bf16 (2^-8 of each). Keys off by h move a score by `d` at most (below), and a probability by the factor e^(2d). So
-    |error| <= 2^-8 |o| + (2 h + 2 d + L 2^-25) max |v|."""
+    keys to fp16 (2^-11 of each, 2^-25 of the largest of 128), probabilities and values to fp16 too (2^-11), or bf16 (2^-8) where rows of a page lie outside
+    fp16's range (`wide`): h. Keys off by 2^-11 move a score by `d` at most (below), and a probability by the factor e^(2d).
+    So |error| <= 2^-8 |o| + (2 h + 2 d + L 2^-25) max |v|."""
     want = ref.attention(q, K, V, cached, scale, amask)
-    L, h = K.shape[0], 2.0 ** -8 if q.shape[0] * (q.shape[1] // K.shape[1]) > 64 or many else 2.0 ** -11
+    of_many = q.shape[0] * (q.shape[1] // K.shape[1]) > 64 or many
+    L, h = K.shape[0], 2.0 ** -8 if of_many and wide else 2.0 ** -11
     fin = torch.where(K.isfinite(), K, torch.zeros_like(K)).double()
     # sum of |q k| h over hd independent roundings: the root of their squares, times six, is never reached
-    d = 6 * h * abs(scale) * float((q.double() ** 2).amax()) ** 0.5 * float((fin ** 2).sum(-1).amax()) ** 0.5
+    d = 6 * 2.0 ** -11 * abs(scale) * float((q.double() ** 2).amax()) ** 0.5 * float((fin ** 2).sum(-1).amax()) ** 0.5
     vmax = float(torch.where(V.isfinite(), V, torch.zeros_like(V)).abs().amax())
     tol = want.abs() * 2.0 ** -8 + (2 * h + 2 * d + L * 2.0 ** -25) * vmax
     assert torch.equal(out.isnan(), want.isnan())
@@ -317,7 +319,7 @@ def test_large_values_of_small_weight_leave_the_others_as_they_are(new, at):
     # what the row adds is below 2^-40: the tolerance is that of the other rows
     V2 = V.clone()
     V2[at] = 0
-    check_attention(out, q, K, V2, cached, 1.0)
+    check_attention(out, q, K, V2, cached, 1.0, wide=True)
 
 
 def test_many_rows_in_pieces_of_every_size():
