@@ -1,14 +1,17 @@
 // Attention of many query rows over the paged 4-bit cache on the 5th-generation tensor cores (tcgen05): prompts and large trees.
 //
 // A CTA takes 256 query rows (row = token * R + head of the group) of a sequence and kv head as two tiles of 128, and its task's positions in steps of
-// 128 (two pages). Per step and tile: S[128 rows][128 positions] = Q K^T into tensor memory, softmax by a warpgroup (a thread a row: no shuffles), P as bf16 back
+// 128 (two pages). Per step and tile: S[128 rows][128 positions] = Q K^T into tensor memory, softmax by a warpgroup (a thread a row: no shuffles), P back
 // into tensor memory over S, O[128][HD] += P V. Tensor pipe and exponentials (16 a clock and SM) need the same 1024 clocks a tile and step at heads of 128, so the two
-// tiles take turns: one multiplies while the other exponentiates. Keys and values are dequantised once for both tiles by eight warps into the K-major
+// tiles take turns: one multiplies while the other exponentiates. Keys and values are dequantised once for both tiles by six warps into the K-major
 // 128-byte-swizzle layout that the MMA reads, K as [position][dim], V as [dim][position], each number (nib - 8) s + z rounded once. (Operands nib - 8, with s and z in the
 // softmax as kv4_attn_few has them, would be exact, but cost the softmax, which is what bounds this kernel, twice its instructions.) All operands are fp16, half a step
-// 2^-11: K times a power of two per step (2^-25 of the largest key of its 128 positions at the smallest), Q times one per row, P times 2^7, V as it is. A page
-// whose rows of V do not all lie within fp16's range has its V and P in bf16, half a step 2^-8: there rows of any size stand side by side, whatever their
-// weight. (With bf16 operands throughout, outputs were off by 0.0044 of their 2-norm; now 0.0017, the rounding of the output itself.) Sums and maxima are fp32.
+// 2^-11: K times a power of two per step (2^-25 of the largest key of its 128 positions at the smallest), Q times one per row, P times 2^7, V as it is. A page whose
+// rows of V have bounds 8 |s| + |z| outside [2^-10, 2^15) has its V and P in bf16, half a step 2^-8: there rows of any size stand side by side, whatever their weight.
+// (With bf16 operands throughout 1000 tokens of 32 heads of 128 behind 7011 took 152 us, but outputs were off by 0.0044 of their 2-norm; now 172 us and 0.0017, which is the
+// rounding of the output itself. Of the 20 us half are the two forms of P, the rest the factors' conversion. Tried and slower: factors converted in place by the warp
+// that brings the pages, 184 us, as it has no more than a step's time; bf16 for the rest of a task from the first such page on, two loops, 169 us but 14.0 for 13.6 us of a
+// tree of 26.) Sums and maxima are fp32.
 // The maximum is moved, and O rescaled, only when a score exceeds it by more than 2^8.
 // Warps: 0..3 and 4..7 softmax of tiles 0 and 1 (and Q in, O out), 8..13 dequantise, 14 brings pages (one bulk copy each), 15 issues MMAs.
 #pragma once
@@ -317,7 +320,27 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
         }
         return (unsigned long long)bad[0] | (unsigned long long)bad[1] << 32;
       };
-      const unsigned long long bad0 = none0 ? 0 : look(rec0, left0, wide0), bad1 = none1 ? 0 : look(rec1, left1, wide1);
+      // The usual case at a glance: whole pages, all factors within narrower bounds than that: s of V from 2^-13 to below 2^11, |z| below 2^14, no NaN and no infinity of K.
+      unsigned long long bad0 = 0, bad1 = 0;
+      {
+        const uint8_t* at = rec0 + (lane >> 4) * C::BLOCK + (lane & 15) * 4;
+        uint32_t km = 0, vm = 0, vs = 0xffffu;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const uint32_t a = *reinterpret_cast<const uint32_t*>(at + (k >> 1) * REC + 2 * (k & 1) * C::BLOCK + C::KSZ) & 0x7fff7fffu,
+                         c = *reinterpret_cast<const uint32_t*>(at + (k >> 1) * REC + 2 * (k & 1) * C::BLOCK + C::VSZ) & 0x7fff7fffu;
+          km = __vmaxu2(km, a);
+          vm = __vmaxu2(vm, c);
+          vs = min(vs, c & 0xffffu);
+        }
+        const bool usual = __vmaxu2(km, 0x7e007e00u) == 0x7e007e00u && __vmaxu2(vm, 0x467f44ffu) == 0x467f44ffu && vs >= 0x3900u;
+        if (__all_sync(0xffffffffu, usual) && !none0 && !none1 && left1 >= kPage) {
+          kmost = __float_as_uint(fmaf(8.f, bflo(km), bfhi(km)));
+        } else {
+          if (!none0) bad0 = look(rec0, left0, wide0);
+          if (!none1) bad1 = look(rec1, left1, wide1);
+        }
+      }
       const float2 kp = pow2_for(__uint_as_float(__reduce_max_sync(0xffffffffu, kmost)));          // the largest into [2^14, 2^15)
       kf = kp.x;
       const bool special = none0 || bad0 || bad1 || left1 < kPage || wide0 || wide1;
@@ -471,28 +494,33 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       }
       const uint64_t cs2 = f32x2(c2, c2), m2 = f32x2(kManyLift - m, kManyLift - m);
       uint64_t sum[4] = {0, 0, 0, 0};
-      auto powers = [&](int c, auto wide) {                      // P of 32 positions
-        uint32_t o[16];
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const float2 y = f32x2_of(fma_f32x2(f32x2(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), cs2, m2));
-          const float a = ex2(y.x), d = ex2(y.y);
-          sum[e & 3] = add_f32x2(sum[e & 3], f32x2(a, d));
-          if (decltype(wide)::value) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[e]) : "f"(d), "f"(a));
-          else o[e] = cvt_f16x2(a, d);
-        }
-        tc_st16(ts + c * 16, o);
-      };
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        if (gone >> h & 4) {
-          powers(2 * h, std::true_type());
-          powers(2 * h + 1, std::true_type());
+#pragma unroll
+        for (int c = 2 * h; c < 2 * h + 2; c++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const float2 y = f32x2_of(fma_f32x2(f32x2(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), cs2, m2));
+            const float a = ex2(y.x), d = ex2(y.y);
+            sum[e & 3] = add_f32x2(sum[e & 3], f32x2(a, d));
+            v[c][2 * e] = __float_as_uint(a);
+            v[c][2 * e + 1] = __float_as_uint(d);
+          }
+        uint32_t o[2][16];
+        if (gone >> h & 4) {                                     // (the conversions alone apart: with the exponentials in both branches heads of 64 took 244 for 235 us)
+#pragma unroll
+          for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[c][e]) : "f"(__uint_as_float(v[2 * h + c][2 * e + 1])), "f"(__uint_as_float(v[2 * h + c][2 * e])));
         } else {
-          powers(2 * h, std::false_type());
-          powers(2 * h + 1, std::false_type());
+#pragma unroll
+          for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[c][e] = cvt_f16x2(__uint_as_float(v[2 * h + c][2 * e]), __uint_as_float(v[2 * h + c][2 * e + 1]));
         }
-        tc_st_wait();                                            // a page's half of P is there
+        tc_st16(ts + 2 * h * 16, o[0]);
+        tc_st16(ts + 2 * h * 16 + 16, o[1]);
+        tc_st_wait();                                          // a page's half of P is there
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * t + h]);

@@ -287,6 +287,36 @@ def test_values_whose_scales_span_many_powers_of_two():
         assert out.isfinite().all()
 
 
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("kp,vp", [(0, -30), (0, -12), (0, 16), (0, 60), (40, 0), (-40, 0), (60, 90)])
+def test_keys_and_values_of_any_size(new, kp, vp):
+    """Keys 2^kp and values 2^vp times the usual, queries 2^-kp times: the same probabilities, values within fp16's range and outside it."""
+    hd, nkv, nh, cached = 128, 2, 8, 300
+    n = cached + new
+    c = make([n], nkv, hd, base=None, garbage=True)
+    c.append(0, rows(51, n, nkv, hd, 2.0 ** kp), rows(52, n, nkv, hd, 2.0 ** vp), 0)
+    K, V = c.read(0, n, 0)
+    q = rows(53, new, nh, hd, 1.5 * 2.0 ** -kp)
+    out = c.attend(0, q, cached)
+    c.check()
+    check_attention(out, q, K, V, cached, hd ** -0.5, wide=vp != 0)
+
+
+def test_one_page_of_a_step_outside_the_range_of_the_other():
+    """Pages of 64 positions whose values are 1, 2^-25, 2^17 and 0 times the usual, ends of the cache at every one of them."""
+    hd, nkv, nh, new = 64, 1, 2, 64
+    size = torch.tensor([1, 2.0 ** -25, 2.0 ** 17, 0, 2.0 ** -25, 1, 0, 2.0 ** 17, 1, 0], device=DEV).repeat_interleave(64)
+    n = size.numel()
+    for page in range(n // 64 - 1):
+        c = make([n], nkv, hd, base=None, garbage=True)
+        q, k, v = rows(61, new, nh, hd), rows(62, n, nkv, hd), (rows(63, n, nkv, hd).float() * size[:, None, None]).bfloat16()
+        c.append(0, k, v, 0)
+        out = c.attend(0, q, page * 64 + 64)      # the next page's tokens are the queries: the chain mask
+        c.check()
+        K, V = (x[:page * 64 + 128] for x in c.read(0, n, 0))
+        check_attention(out, q, K, V, page * 64 + 64, hd ** -0.5, wide=True)
+
+
 @pytest.mark.parametrize("hd", [64, 80, 128])
 def test_a_none_of_a_later_step_stays_there(hd):
     """Steps of 128 positions follow one another while the softmax of earlier ones runs: a value that is none in the third is not held against the first."""
