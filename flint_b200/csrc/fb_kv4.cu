@@ -55,7 +55,7 @@ int done(cudaError_t e) { return e == cudaSuccess ? FB_OK : FB_ERR_CUDA; }
 // second launch that joins them, beyond that. (With one CTA of 16-row groups per SM the GPU holds 15 clusters of 8, but 36 of 4.) One sequence, eight
 // kv heads, cluster / second launch: 1000 positions 5.5 / 8.2, 4000 6.7 / 8.5, 32768 20.5 / 13.1 (heads of 80). Of a batch no positions are shared until a
 // warp would have more than 12 units: 48 sequences of up to 2000 positions 17.8 / 22.7, 24 of up to 8000 51 / 18.3 (over 148 parts; over 296 22.1).
-// Many: a step of 128 positions takes 2.5 us (1.6 with one tile of rows), a task about two steps more, the second launch 5 us and what the partials take to
+// Many: a step of 128 positions takes about 2.5 us (1.6 with one tile of rows), a task about two steps more, the second launch 5 us and what the partials take to
 // write and read; the number of parts with the smallest sum is taken. 1000 tokens behind 7011 positions, 160 items on 148 SMs: whole 253, four
 // parts 216; 128 items: whole 160, two parts 197. 61-node tree, eight items: whole 71, eight parts 28.4, 24 parts 42.
 struct Kv4Geometry { int rows; int64_t groups, ctas; int nsplit, slots, chunk; };

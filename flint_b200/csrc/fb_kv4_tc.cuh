@@ -8,10 +8,9 @@
 // softmax as kv4_attn_few has them, would be exact, but cost the softmax, which is what bounds this kernel, twice its instructions.) All operands are fp16, half a step
 // 2^-11: K times a power of two per step (2^-25 of the largest key of its 128 positions at the smallest), Q times one per row, P times 2^7, V as it is. A page whose
 // rows of V have bounds 8 |s| + |z| outside [2^-10, 2^15) has its V and P in bf16, half a step 2^-8: there rows of any size stand side by side, whatever their weight.
-// (With bf16 operands throughout 1000 tokens of 32 heads of 128 behind 7011 took 152 us, but outputs were off by 0.0044 of their 2-norm; now 172 us and 0.0017, which is the
-// rounding of the output itself. Of the 20 us half are the two forms of P, the rest the factors' conversion. Tried and slower: factors converted in place by the warp
-// that brings the pages, 184 us, as it has no more than a step's time; bf16 for the rest of a task from the first such page on, two loops, 169 us but 14.0 for 13.6 us of a
-// tree of 26.) Sums and maxima are fp32.
+// (With bf16 operands throughout 1000 tokens of 32 heads of 128 behind 7011 took 152 us, but outputs were off by 0.0044 of their 2-norm; now 166 us, 743 TFLOP/s, and 0.0017,
+// which is the rounding of the output itself. What is dearer is the factors' look and conversion, and P's second form. Tried and slower: factors converted in place by the
+// warp that brings the pages, 184 us, as it has no more than a step's time; P in either form behind a branch, 172 us.) Sums and maxima are fp32.
 // The maximum is moved, and O rescaled, only when a score exceeds it by more than 2^8.
 // Warps: 0..3 and 4..7 softmax of tiles 0 and 1 (and Q in, O out), 8..13 dequantise, 14 brings pages (one bulk copy each), 15 issues MMAs.
 #pragma once
@@ -495,35 +494,46 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       const uint64_t cs2 = f32x2(c2, c2), m2 = f32x2(kManyLift - m, kManyLift - m);
       uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
+      for (int c = 0; c < 4; c++) {
+        uint32_t o[16];
 #pragma unroll
-        for (int c = 2 * h; c < 2 * h + 2; c++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            const float2 y = f32x2_of(fma_f32x2(f32x2(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), cs2, m2));
-            const float a = ex2(y.x), d = ex2(y.y);
-            sum[e & 3] = add_f32x2(sum[e & 3], f32x2(a, d));
-            v[c][2 * e] = __float_as_uint(a);
-            v[c][2 * e + 1] = __float_as_uint(d);
-          }
-        uint32_t o[2][16];
-        if (gone >> h & 4) {                                     // (the conversions alone apart: with the exponentials in both branches heads of 64 took 244 for 235 us)
-#pragma unroll
-          for (int c = 0; c < 2; c++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[c][e]) : "f"(__uint_as_float(v[2 * h + c][2 * e + 1])), "f"(__uint_as_float(v[2 * h + c][2 * e])));
-        } else {
-#pragma unroll
-          for (int c = 0; c < 2; c++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[c][e] = cvt_f16x2(__uint_as_float(v[2 * h + c][2 * e]), __uint_as_float(v[2 * h + c][2 * e + 1]));
+        for (int e = 0; e < 16; e++) {
+          const float2 y = f32x2_of(fma_f32x2(f32x2(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), cs2, m2));
+          const float a = ex2(y.x), d = ex2(y.y);
+          sum[e & 3] = add_f32x2(sum[e & 3], f32x2(a, d));
+          o[e] = cvt_f16x2(a, d);
+          v[c][2 * e] = __float_as_uint(a);
+          v[c][2 * e + 1] = __float_as_uint(d);
         }
-        tc_st16(ts + 2 * h * 16, o[0]);
-        tc_st16(ts + 2 * h * 16 + 16, o[1]);
-        tc_st_wait();                                          // a page's half of P is there
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * t + h]);
+        tc_st16(ts + c * 16, o);
+        if (c & 1) {                                             // a page's half of P is there
+          tc_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0 && !(gone >> (c >> 1) & 4)) mbar_arrive(&p_full[2 * t + (c >> 1)]);
+        }
+      }
+      if (gone & 12) {                                           // as bf16, by way of columns whose scores have been read: the usual path runs straight on (its second half's
+                                                                 // exponentials during the first half's store)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          if (!(gone >> h & 4)) continue;
+          tc_st32(ts + 64, v[2 * h]);
+          tc_st32(ts + 96, v[2 * h + 1]);
+          tc_st_wait();
+#pragma unroll 1
+          for (int k = 0; k < 64; k += 8) {
+            uint32_t x[8];
+            tc_ld8(ts + 64 + k, x);
+            tc_ld_wait();
+            tc_st4(ts + h * 32 + k / 2, pack_bf16(__uint_as_float(x[0]), __uint_as_float(x[1])), pack_bf16(__uint_as_float(x[2]), __uint_as_float(x[3])),
+                   pack_bf16(__uint_as_float(x[4]), __uint_as_float(x[5])), pack_bf16(__uint_as_float(x[6]), __uint_as_float(x[7])));
+          }
+          tc_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * t + h]);
+        }
       }
       {
         const float2 y = f32x2_of(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])));
