@@ -30,7 +30,7 @@ struct Kv4Many {
   static constexpr int ND = 4;                                              // steps whose notes are kept: softmax may be at i when step i + 2 is dequantised
   static constexpr int NR = 4;                                              // pages: two being dequantised, two on their way
   static constexpr int Q = 0, K = Q + 2 * QT, V = K + 2 * KT, RAW = V + 4 * VT, BAR = RAW + NR * REC;
-  static constexpr int BARS = 2 * NR + 17, TOTAL = BAR + BARS * 8 + 2 * ND * 8 + (2 + 5 + NR + 2 * ND) * 4;       // barriers, then what stands behind them in the kernel
+  static constexpr int BARS = 2 * NR + 17, TOTAL = BAR + BARS * 8 + 2 * ND * 8 + (2 + 2 + NR + 2 * ND) * 4;       // barriers, then what stands behind them in the kernel
   static constexpr int T_S = 0, T_O = 256, TCOLS = 512;                     // tensor memory columns: two S / P, two O
   static_assert(TOTAL <= 227 * 1024 && T_O + 2 * HD <= TCOLS && QT % 1024 == 0 && VT % 1024 == 0 && RAW % 16 == 0 && REC % 16 == 0, "plan");
 };
@@ -80,14 +80,13 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   return d;
 }
 
-// after a failure: the copies and MMAs in flight
+// after a failure: the copies in flight, and the MMAs, half a step's that nothing was committed for among them: one more commit behind all of them
 template <int NR>
-inline __device__ __noinline__ void many_drain(uint64_t* raw_full, uint64_t* s_full, uint64_t* pv_done, volatile int* s_issued) {
+inline __device__ __noinline__ void many_drain(uint64_t* raw_full, uint64_t* pv_done, volatile int* s_issued) {
   drain_ring<NR>(raw_full, (uint32_t)s_issued[0]);
-  for (int t = 0; t < 2; t++) {
-    if (s_issued[1 + t]) drain_phase(&s_full[t], (uint32_t)(s_issued[1 + t] - 1) & 1u);
-    if (s_issued[3 + t]) drain_phase(&pv_done[t], (uint32_t)(s_issued[3 + t] - 1) & 1u);
-  }
+  if (elect_one()) tc_commit(pv_done);
+  __syncwarp();
+  drain_phase(pv_done, (uint32_t)s_issued[1] & 1u);
   __syncwarp();
 }
 
@@ -104,8 +103,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
   unsigned long long* s_bad = reinterpret_cast<unsigned long long*>(bars + M::BARS);   // [ND steps][2 pages] positions whose V is NaN
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_bad + 2 * M::ND);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-  volatile int* s_issued = s_abort + 1;                          // [5] pages, QK of tiles 0 and 1, PV of tiles 0 and 1
-  volatile int* s_none = s_issued + 5;                           // [NR] the page does not exist
+  volatile int* s_issued = s_abort + 1;                          // [2] pages, PV of tile 0
+  volatile int* s_none = s_issued + 2;                           // [NR] the page does not exist
   volatile int* s_gone = s_none + NR;                            // [ND steps] bit p: page p of the step does not exist, bit 2 + p: it is wide
   volatile float* s_kscale = reinterpret_cast<volatile float*>(s_gone + M::ND);  // [ND steps] inverse of the power of two of the keys
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -123,7 +122,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
     }
     mbar_init(q_full, 4 * tiles);
     *s_abort = 0;
-    for (int i = 0; i < 5; i++) s_issued[i] = 0;
+    s_issued[0] = s_issued[1] = 0;
     mbar_fence_init();
   }
   if (warp == 15) {
@@ -183,7 +182,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
         if (t == tiles - 1) tc_commit(&k_empty[i & 1]);
       }
       __syncwarp();
-      if (lane == 0) s_issued[1 + t] = i + 1;
     };
     auto pv = [&](auto tile, auto part, int i) {                 // of the step's first or second page
       constexpr int t = decltype(tile)::value, h = decltype(part)::value;
@@ -200,7 +198,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
         }
       }
       __syncwarp();
-      if (h && lane == 0) s_issued[3 + t] = i + 1;
+      if (t == 0 && h && lane == 0) s_issued[1] = i + 1;
     };
     auto wait = [&](uint64_t* bar, int i, int where) {           // phase i of a barrier
       ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, (uint32_t)i & 1u, wc, W_FULL, where));
@@ -578,7 +576,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
   tc_fence_before();
   __syncthreads();
   if (warp == 15) {
-    if (*s_abort) many_drain<NR>(raw_full, s_full, pv_done, s_issued);
+    if (*s_abort) many_drain<NR>(raw_full, pv_done, s_issued);
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(M::TCOLS));
   }
 }

@@ -228,3 +228,30 @@ def test_chat_on_four_bits():
                          text=True, timeout=300)
     assert run.returncode == 0, run.stderr[-500:]
     assert run.stdout.count("8 tokens") == 2
+
+
+@pytest.mark.parametrize("name,M,pos", [("tiny", 1, 0), ("tiny", 3, 600), ("tiny", 40, 0), ("tiny", 300, 0), ("tiny", 16, 600), ("llama-8b-class", 1, 3000),
+                                        ("llama-8b-class", 26, 1500), ("llama-8b-class", 61, 700), ("llama-8b-class", 200, 700)])
+def test_passes_that_give_up_leave_nothing_behind(name, M, pos):
+    """A wait limit of 0: every launch ends, after what it has in flight (that wait has its own limit), the status says time-out or, if every wait happened to be
+    satisfied, nothing, and the next clean pass gives the bits of the first."""
+    cfg = ModelArgs.from_name(name)
+    if name != "tiny":
+        cfg.n_layer, cfg.vocab_size = 1, 512
+    eng = DecodeEngine(cfg, packing.synth_packed(cfg, 0, device=DEV), max_seq=pos + 512, kv_bits=4)
+    g = torch.Generator(device=DEV).manual_seed(pos)
+    for layer in range(cfg.n_layer if pos else 0):
+        k, v = (torch.randn(pos, cfg.n_local_heads, cfg.head_dim, generator=g, device=DEV).bfloat16() for _ in range(2))
+        eng.cache.append(layer, k, v, 0)
+    toks = torch.randint(0, cfg.vocab_size, (M,), generator=torch.Generator().manual_seed(M), dtype=torch.int32).to(DEV)
+    run = (lambda: eng.decode(17, pos).clone()) if M == 1 else (lambda: (eng.verify if M <= 64 else eng.prefill)(toks, pos)[0])
+    want = run()
+    eng.check()
+    for _ in range(8):
+        eng.set_option(0, 0)
+        run()
+        assert eng.status()["code"] in (_lib.FB_OK, _lib.FB_ERR_TIMEOUT)
+        eng.set_option(0, 4000000)
+        again = run()
+        eng.check()
+        assert torch.equal(want, again)
