@@ -457,6 +457,74 @@ def test_a_step_of_decoding_from_a_captured_graph():
                 check_attention(got[s][i][b:b + 1], q, K[:i + 1 + 3 * b], V[:i + 1 + 3 * b], i + 3 * b, hd ** -0.5)
 
 
+def test_sequences_that_share_their_first_pages():
+    """A common prompt: three sequences whose tables name the same pages at first, and their own behind them."""
+    hd, nkv, nh, common = 80, 2, 8, 192
+    own = [5, 70, 130]
+    table = torch.full((3, 6), -1, dtype=torch.int32)
+    table[:, :3] = torch.tensor([4, 0, 9])
+    at = iter([1, 2, 3, 5, 6, 7, 8])
+    for b, n in enumerate(own):
+        for i in range((n + 63) // 64):
+            table[b, 3 + i] = next(at)
+    c = KvCache4(1, 10, nkv, hd, table.to(DEV), rope_base=None)
+    k, v = rows(1, common, nkv, hd), rows(2, common, nkv, hd)
+    c.append(0, k, v, ints(0, 0, 0), start=ints(0, common, common, common))         # once, by the first
+    starts = ints(0, *torch.tensor(own).cumsum(0).tolist())
+    c.append(0, rows(3, sum(own), nkv, hd), rows(4, sum(own), nkv, hd), ints(*[common] * 3), start=starts)
+    for new in (1, 5):
+        q = rows(5, 3 * new, nh, hd)
+        cached = [common + n - new for n in own]
+        out = c.attend(0, q, ints(*cached), start=ints(0, new, 2 * new, 3 * new), max_new=new)
+        for b in range(3):
+            one = KvCache4(1, 10, nkv, hd, c.table[b:b + 1].contiguous(), pool=c.pool, rope_base=None)
+            K, V = one.read(0, cached[b] + new, 0)
+            check_attention(out[b * new:(b + 1) * new], q[b * new:(b + 1) * new], K, V, cached[b], hd ** -0.5)
+    c.check()
+
+
+@pytest.mark.parametrize("new,cached", [(1, 9000), (40, 3000), (300, 600)])
+def test_calls_on_two_streams_at_once_have_their_own_scratch(new, cached):
+    hd, nkv, nh = 128, 2, 8
+    c, K, V, q, _ = filled([cached], [new], nh, nkv, hd, seed=9)
+    q2 = rows(77, new, nh, hd)
+    want = c.attend(0, q, cached), c.attend(0, q2, cached)
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = [], []
+    for _ in range(20):
+        for i, x in enumerate((q, q2)):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(c.attend(0, x, cached))
+    torch.cuda.synchronize()
+    c.check()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in outs[i])
+
+
+def test_a_captured_prompt_over_lengths_on_the_gpu():
+    """Two graphs, captured one after the other and replayed in turn while the lengths that they read change."""
+    hd, nkv, nh, new = 64, 2, 8, 40
+    c, K, V, q, _ = filled([900], [new], nh, nkv, hd, seed=12)
+    cached = ints(900)
+    c.attend(0, q, cached)                                       # (first use sets the kernels up)
+    torch.cuda.synchronize()
+    q2 = rows(78, new, nh, hd)
+    graphs, outs = [], []
+    for x in (q, q2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(c.attend(0, x, cached))
+        graphs.append(g)
+    for n in (900, 0, 63, 500, 64):
+        cached.fill_(n)
+        for g in graphs:
+            g.replay()
+        for x, out in zip((q, q2), outs):
+            check_attention(out, x, K[0][:n + new], V[0][:n + new], n, hd ** -0.5)
+    c.check()
+
+
 def test_nothing_to_do():
     c = make([64], 2, 64)
     empty = torch.empty(0, 2, 64, dtype=torch.bfloat16, device=DEV)
