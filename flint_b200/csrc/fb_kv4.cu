@@ -55,30 +55,36 @@ int done(cudaError_t e) { return e == cudaSuccess ? FB_OK : FB_ERR_CUDA; }
 // second launch that joins them, beyond that. (With one CTA of 16-row groups per SM the GPU holds 15 clusters of 8, but 36 of 4.) One sequence, eight
 // kv heads, cluster / second launch: 1000 positions 5.5 / 8.2, 4000 6.7 / 8.5, 32768 20.5 / 13.1 (heads of 80). Of a batch no positions are shared until a
 // warp would have more than 12 units: 48 sequences of up to 2000 positions 17.8 / 22.7, 24 of up to 8000 51 / 18.3 (over 148 parts; over 296 22.1).
-// Many: a step of 128 positions takes about 2.5 us (1.6 with one tile of rows), a task about two steps more, the second launch 5 us and what the partials take to
-// write and read; the number of parts with the smallest sum is taken. 1000 tokens behind 7011 positions, 160 items on 148 SMs: whole 253, four
-// parts 216; 128 items: whole 160, two parts 197. 61-node tree, eight items: whole 71, eight parts 28.4, 24 parts 42.
+// Many: a task has 128 or 256 query rows. A step of 128 positions takes about 2.5 us (1.6 with one tile of 128 rows), a task about two steps more, the second launch 5 us and what the
+// partials take to write and read; rows and parts of the smallest sum are taken. 1000 tokens of 4 heads behind 7011 positions, 160 items of 256 rows on 148 SMs: whole
+// 253, four parts 216; 128 items: whole 160, two parts 197. 61-node tree of 4 heads behind 3001: eight items of 256 rows whole 71, eight parts 28.3, 24 parts 42; sixteen of
+// 128 rows in eight parts 23.8. A prompt of 200 tokens: 12.4 with 256 rows, 10.5 with 128.
 struct Kv4Geometry { int rows; int64_t groups, ctas; int nsplit, slots, chunk; };
 Kv4Geometry few_geometry(int n_seq, int n_tokens, int nkv, int r, int max_new, int max_len, int sms) {
   Kv4Geometry g{(int64_t)max_new * r <= 8 ? 8 : 16, 0, 0, 1, 0, 8};
-  if ((int64_t)max_new * r > kFewRows) g.rows = kManyRows;
-  g.groups = n_seq == 1 ? ((int64_t)n_tokens * r + g.rows - 1) / g.rows : (int64_t)n_tokens * r / g.rows + n_seq;
-  const int64_t units = ((int64_t)max_len + 31) / 32, items = g.groups * nkv;
-  if (g.rows == kManyRows) {
+  auto groups_of = [&](int rows) { return n_seq == 1 ? ((int64_t)n_tokens * r + rows - 1) / rows : (int64_t)n_tokens * r / rows + n_seq; };
+  const bool many = (int64_t)max_new * r > kFewRows;
+  const int64_t units = ((int64_t)max_len + 31) / 32, steps = ((int64_t)max_len + kManyStep - 1) / kManyStep;
+  if (many) {
     g.chunk = 1;
-    const int64_t steps = ((int64_t)max_len + kManyStep - 1) / kManyStep;
-    const double step_us = (int64_t)max_new * r > 128 ? 2.5 : 1.6;
     double best = 0;
-    for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24}) {
-      if (parts > steps || (parts > 1 && items * parts > 3 * sms)) break;
-      const int64_t per = (steps + parts - 1) / parts, tasks = items * ((steps + per - 1) / per);
-      const double us = (double)((tasks + sms - 1) / sms) * (double)(per + 2) * step_us + (parts > 1 ? 5.0 + (double)tasks * kManyRows * 1056 / 3e6 : 0.0);
-      if (parts == 1 || us < best) { best = us; g.slots = parts > 1 ? (int)(items * parts) : 0; }
+    for (int rows : {kManyRows / 2, kManyRows}) {
+      const double step_us = rows == kManyRows && (int64_t)max_new * r > kManyRows / 2 ? 2.5 : 1.6;
+      const int64_t items = groups_of(rows) * nkv;
+      for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24}) {
+        if (parts > steps || (parts > 1 && items * parts > 3 * sms)) break;
+        const int64_t per = (steps + parts - 1) / parts, tasks = items * ((steps + per - 1) / per);
+        const double us = (double)((tasks + sms - 1) / sms) * (double)(per + 2) * step_us + (parts > 1 ? 5.0 + (double)tasks * rows * 1056 / 3e6 : 0.0);
+        if (best == 0 || us < best) { best = us; g.rows = rows; g.slots = parts > 1 ? (int)(items * parts) : 0; }
+      }
     }
-  } else if (n_seq == 1) {
+  }
+  g.groups = groups_of(g.rows);
+  const int64_t items = g.groups * nkv;
+  if (!many && n_seq == 1) {
     while (g.nsplit < 8 && items * g.nsplit * 2 <= (g.nsplit == 4 ? sms * 2 / 3 : sms) && units >= g.nsplit * 2 * 4) g.nsplit *= 2;
     if (units > (int64_t)6 * kFewWarps * g.nsplit && items * g.nsplit <= sms) { g.nsplit = 1; g.slots = 2 * sms; }
-  } else if (units > 12 * kFewWarps && items <= 8 * (int64_t)sms) {
+  } else if (!many && units > 12 * kFewWarps && items <= 8 * (int64_t)sms) {
     g.slots = sms;
   }
   g.ctas = items + g.slots;
@@ -118,28 +124,29 @@ cudaError_t launch_few(Kv4Attend p, const Kv4Geometry& g, cudaStream_t st) {
   return launch_pdl(kv4_join<HD, F::ROWS, F::U, 1>, dim3((unsigned)g.groups, (unsigned)p.S.nkv, F::ROWS / 8), dim3(256), 0, st, p);
 }
 // kv4_attn_many deals its registers out anew and counts on 128 a thread at launch
-template <int HD>
+template <int HD, int ROWS>
 bool configured_many() {
   static int regs = 0;
   cudaFuncAttributes a;
-  if (!regs && cudaFuncGetAttributes(&a, kv4_attn_many<HD>) == cudaSuccess) regs = a.numRegs;
+  if (!regs && cudaFuncGetAttributes(&a, kv4_attn_many<HD, ROWS>) == cudaSuccess) regs = a.numRegs;
   return regs == 128;
 }
-template <int HD>
+template <int HD, int ROWS>
 cudaError_t launch_many(Kv4Attend p, const Kv4Geometry& g, cudaStream_t st) {
   static bool done[64] = {};
   p.nsplit = 1; p.slots = g.slots; p.chunk = g.chunk;
   if (g.groups > 0x7fffffff || g.ctas > 0x7fffffff) return cudaErrorInvalidValue;
-  if (g.groups > 0 && !configured_many<HD>()) return cudaErrorInvalidConfiguration;
-  cudaError_t e = configure_few(kv4_attn_many<HD>, Kv4Many<HD>::TOTAL, done);
-  if (e == cudaSuccess) e = launch_pdl(kv4_attn_many<HD>, dim3((unsigned)g.ctas), dim3(kManyThreads), (size_t)Kv4Many<HD>::TOTAL, st, p);
+  if (g.groups > 0 && !configured_many<HD, ROWS>()) return cudaErrorInvalidConfiguration;
+  cudaError_t e = configure_few(kv4_attn_many<HD, ROWS>, Kv4Many<HD>::TOTAL, done);
+  if (e == cudaSuccess) e = launch_pdl(kv4_attn_many<HD, ROWS>, dim3((unsigned)g.ctas), dim3(kManyThreads), (size_t)Kv4Many<HD>::TOTAL, st, p);
   if (e == cudaSuccess && g.slots)
-    e = launch_pdl(kv4_join<HD, kManyRows, kManyStep, 1>, dim3((unsigned)g.groups, (unsigned)p.S.nkv, kManyRows / 8), dim3(256), 0, st, p);
+    e = launch_pdl(kv4_join<HD, ROWS, kManyStep, 1>, dim3((unsigned)g.groups, (unsigned)p.S.nkv, ROWS / 8), dim3(256), 0, st, p);
   return e;
 }
 template <int HD>
 cudaError_t launch_attend(const Kv4Attend& p, const Kv4Geometry& g, cudaStream_t st) {
-  return g.rows == kManyRows ? launch_many<HD>(p, g, st) : (g.rows == 8 ? launch_few<HD, 1, kFewWarps>(p, g, st) : launch_few<HD, 2, kFewWarps>(p, g, st));
+  if (g.rows >= kManyRows / 2) return g.rows == kManyRows ? launch_many<HD, kManyRows>(p, g, st) : launch_many<HD, kManyRows / 2>(p, g, st);
+  return (g.rows == 8 ? launch_few<HD, 1, kFewWarps>(p, g, st) : launch_few<HD, 2, kFewWarps>(p, g, st));
 }
 
 }  // namespace

@@ -1,6 +1,6 @@
 // Attention of many query rows over the paged 4-bit cache on the 5th-generation tensor cores (tcgen05): prompts and large trees.
 //
-// A CTA takes 256 query rows (row = token * R + head of the group) of a sequence and kv head as two tiles of 128, and its task's positions in steps of
+// A CTA takes 256 query rows (row = token * R + head of the group) of a sequence and kv head as two tiles of 128 (or 128 rows, where the SMs are not filled otherwise), and its task's positions in steps of
 // 128 (two pages). Per step and tile: S[128 rows][128 positions] = Q K^T into tensor memory, softmax by a warpgroup (a thread a row: no shuffles), P back
 // into tensor memory over S, O[128][HD] += P V. Tensor pipe and exponentials (16 a clock and SM) need the same 1024 clocks a tile and step at heads of 128, so the two
 // tiles take turns: one multiplies while the other exponentiates. Keys and values are dequantised once for both tiles by six warps into the K-major
@@ -90,7 +90,7 @@ inline __device__ __noinline__ void many_drain(uint64_t* raw_full, uint64_t* pv_
   __syncwarp();
 }
 
-template <int HD>
+template <int HD, int ROWS>
 __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend P) {
   using C = Kv4<HD>;
   using M = Kv4Many<HD>;
@@ -110,10 +110,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Kv4Seqs& S = P.S;
   pdl_begin(true);
-  Kv4Task<kManyRows, kManyStep> task;
+  Kv4Task<ROWS, kManyStep> task;
   if (!task.template find<false>(P, blockIdx.x, lane, blockIdx.x == 0 && warp == 0) || (task.n <= 0 && task.parts == 1)) return;
   const Kv4Seq& seq = task.seq;
-  const int rows = task.rows - task.r0, tiles = rows > 128 ? 2 : 1, n = max(task.n, 0), kvh = task.kvh, total = task.total;
+  const int rows = task.rows - task.r0, tiles = ROWS > 128 && rows > 128 ? 2 : 1, n = max(task.n, 0), kvh = task.kvh, total = task.total;
   if (tid == 0) {
     for (int i = 0; i < NR; i++) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], kManyDequant); }
     for (int i = 0; i < 2; i++) {
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
     if (ok) {
       const float inv = task.parts > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
       uint16_t* out = P.out + (size_t)(seq.first + mq) * P.o_ld + (size_t)head * HD;
-      float* w = task.parts > 1 ? P.work + ((size_t)blockIdx.x * kManyRows + lr) * (HD + 4) : nullptr;
+      float* w = task.parts > 1 ? P.work + ((size_t)blockIdx.x * ROWS + lr) * (HD + 4) : nullptr;
 #pragma unroll 1
       for (int c = 0; c < HD; c += 16) {
         uint32_t v[16];
