@@ -73,7 +73,7 @@ def main():
         respond(model, ids, 8, kw, stream=False)                                  # warm-up: builds the context
         new, dt = respond(model, ids, a.max_new, kw)
         print(f"\n{len(new)} tokens · {len(new) / dt:.1f} tok/s including the {len(ids)}-token prefill "
-              f"({"M-token passes, 4-bit K/V" if a.kv_bits == 4 else "megakernel"} int4, {cfg.n_layer} layers, d {cfg.dim})")
+              f"({'M-token passes, 4-bit K/V' if a.kv_bits == 4 else 'megakernel'} int4, {cfg.n_layer} layers, d {cfg.dim})")
         return
     print("flint_b200 chat on token ids: one line of ids per turn, empty line or EOF to quit.")
     history = []
