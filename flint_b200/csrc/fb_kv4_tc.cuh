@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       }
       const float2 kp = pow2_for(__uint_as_float(__reduce_max_sync(0xffffffffu, kmost)));          // the largest into [2^14, 2^15)
       kf = kp.x;
-      const bool special = none0 || bad0 || bad1 || left1 < kPage || wide0 || wide1;
+      const bool special = none0 || none1 || bad0 || bad1 || left1 < kPage || wide0 || wide1;
       if (dw == 0 && lane == 0) {
         // Their place was step i - 4's: the softmax of that one has read it, as PV of step i - 3 has ended (the wait for V's place of the step before)
         const int note = i & (M::ND - 1);

@@ -1,0 +1,33 @@
+"""GPU: the 4-bit cache where its calls can go wrong: pages that the table does not have, rows that nobody sees, numbers of every size, sequences that cannot be."""
+import pytest
+import torch
+
+from flint_b200 import _lib
+from tests.test_gpu_kv4 import check_attention, make, rows
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("hd", [64, 80, 128])
+@pytest.mark.parametrize("nkv", [2, 148])                   # tasks of a few steps, and of all of them
+@pytest.mark.parametrize("missing", [[1], [2], [5], [7], [2, 3], [4, 7]])
+def test_many_rows_leave_out_pages_that_the_table_does_not_have(hd, nkv, missing):
+    """First and second pages of a step in the middle of a sequence. The places that their copies would go to hold what was there before: page 3's values, which are
+    numbers but none that fp16 has, or whatever shared memory held."""
+    cached, new, nh = 640, 40, 2 * nkv
+    c = make([cached + new], nkv, hd, base=None, garbage=True)
+    k, v = rows(1, cached + new, nkv, hd, 1.3), rows(2, cached + new, nkv, hd)
+    v[192:256] *= 2.0 ** 18
+    c.append(0, k, v, 0)
+    K, V = c.read(0, cached + new, 0)
+    q = rows(3, new, nh, hd, 1.5)
+    seen = torch.ones(cached + new, dtype=torch.bool, device=DEV)
+    for page in missing:
+        seen[64 * page:64 * page + 64] = False
+        c.table[0, page] = -1
+    for _ in range(2):
+        out = c.attend(0, q, cached)
+        st = c.status()
+        assert st["code"] == _lib.FB_ERR_RANGE and st["where"] == 21
+        check_attention(out, q, K[seen], V[seen], cached - 64 * len(missing), hd ** -0.5, wide=True)
