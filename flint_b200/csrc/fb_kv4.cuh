@@ -15,6 +15,7 @@
 #include <type_traits>
 
 #include "fb_common.cuh"
+#include "fb_drain.hpp"
 
 namespace fb {
 

@@ -80,14 +80,12 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   return d;
 }
 
-// after a failure: the copies in flight, and the MMAs, half a step's that nothing was committed for among them: one more commit behind all of them
+// after a failure: the copies in flight, and the MMAs, half a step's that nothing was committed for among them
 template <int NR>
 inline __device__ __noinline__ void many_drain(uint64_t* raw_full, uint64_t* pv_done, volatile int* s_issued) {
   drain_ring<NR>(raw_full, (uint32_t)s_issued[0]);
-  if (elect_one()) tc_commit(pv_done);
-  __syncwarp();
-  drain_phase(pv_done, (uint32_t)s_issued[1] & 1u);
-  __syncwarp();
+  drain_commit_order((uint32_t)s_issued[1], [=](uint32_t parity) { drain_phase(pv_done, parity); __syncwarp(); },
+                     [=] { if (elect_one()) tc_commit(pv_done); __syncwarp(); });
 }
 
 template <int HD, int ROWS>

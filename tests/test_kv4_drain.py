@@ -1,0 +1,63 @@
+"""CPU: what a launch over the 4-bit cache that gives up waits for before it ends (flint_b200/csrc/fb_drain.hpp), run against a model of the barriers in which everything ends
+as late as it can: nothing may be in flight behind it, and no wait may be one that nothing ends."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "flint_b200", "csrc")
+SHIM = """
+#include "fb_drain.hpp"
+typedef void (*Wait)(uint32_t);
+typedef void (*Commit)();
+extern "C" void commits(uint32_t committed, Wait wait, Commit commit) { fb::drain_commit_order(committed, wait, commit); }
+"""
+WAIT, COMMIT = ctypes.CFUNCTYPE(None, ctypes.c_uint32), ctypes.CFUNCTYPE(None)
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    d = tmp_path_factory.mktemp("drain")
+    (d / "drain.cpp").write_text(SHIM)
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", CSRC, "-o", str(d / "drain.so"), str(d / "drain.cpp")])
+    return ctypes.CDLL(str(d / "drain.so"))
+
+
+class Barrier:
+    """Phases 0 .. armed-1 have been issued, 0 .. over-1 of them have ended; a parity wait passes when phase over - 1 has that parity, else the next one ends."""
+
+    def __init__(self, armed=0, over=0):
+        self.armed, self.over, self.hung = armed, over, False
+
+    def wait(self, parity):
+        while (self.over & 1) == parity:
+            if self.over == self.armed:
+                self.hung = True
+                return
+            self.over += 1
+
+    @property
+    def quiet(self):
+        return self.over == self.armed and not self.hung
+
+
+@pytest.mark.parametrize("committed", range(7))
+def test_every_product_has_ended(lib, committed):
+    """The last commit may be under way or over; the one before it is over (a tile's next products wait for it)."""
+    for over in {max(0, committed - 1), committed}:
+        b = Barrier(committed, over)
+        lib.commits(committed, WAIT(b.wait), COMMIT(lambda: setattr(b, "armed", b.armed + 1)))
+        assert b.armed == committed + 1 and b.quiet
+
+
+def test_the_model_shows_the_orders_that_do_not_do():
+    """One more commit and a wait for it alone passes over the commit ahead of it; a wait for both behind it may be one that nothing ends."""
+    b = Barrier(3, 2)
+    b.armed += 1
+    b.wait(1)
+    assert not b.quiet
+    b = Barrier(3, 3)
+    b.armed, b.over = 4, 4
+    b.wait(0)
+    assert b.hung
