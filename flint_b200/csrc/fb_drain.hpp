@@ -8,6 +8,14 @@
 
 namespace fb {
 
+// The last (up to) N of `issued` copies into a ring of N stages: wait(stage, parity). A copy into a stage is issued once the one before it there has ended. Only copies
+// that were issued count: one more, and the oldest is passed over.
+template <int N, class Wait>
+constexpr void drain_ring_order(uint32_t issued, Wait wait) {
+  const uint32_t n = issued < (uint32_t)N ? issued : (uint32_t)N;
+  for (uint32_t k = 1; k <= n; k++) wait((issued - k) % N, ((issued - k) / N) & 1);
+}
+
 // Everything that was issued ahead of one more commit() on a barrier that `committed` commits have armed, the last of which may be under way: that one
 // first, then the new one, which also ends what no commit was issued for.
 template <class Wait, class Commit>

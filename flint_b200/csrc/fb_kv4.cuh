@@ -572,12 +572,12 @@ __global__ void __launch_bounds__(W * 32 + 32) kv4_attn_few(const Kv4Attend P) {
   __syncthreads();
   const WaitCtl wc{S.status, s_abort, P.spin_limit};
   bool ok = true;
-  int issued = 0;                                                // rounds that the copying warp has begun
+  uint32_t issued = 0;                                           // of the copying warp, a lane each: its copies (and pages that are none)
   if (warp == W) {
     int st = 0;
     uint32_t lap = 1;
-    for (; issued < rounds && ok; issued++) {
-      const int i = issued * W + lane;
+    for (int round = 0; round < rounds && ok; round++) {
+      const int i = round * W + lane;
       const bool mine = lane < W && i < n;
       const int now = page;
       if (mine && i + W < n) page = kv4_page(S, b, (u_begin + i + W) * U, true);
@@ -592,6 +592,7 @@ __global__ void __launch_bounds__(W * 32 + 32) kv4_attn_few(const Kv4Attend P) {
             mbar_expect_tx(&full[k], F::STAGE);
             bulk_g2s(sm + k * F::STAGE, kv4_block<HD>(S, now, kvh, (u_begin + i) * U), F::STAGE, &full[k]);
           }
+          issued++;
         }
       }
       ok = __all_sync(0xffffffffu, ok);
@@ -847,8 +848,7 @@ __global__ void __launch_bounds__(W * 32 + 32) kv4_attn_few(const Kv4Attend P) {
       }
   __syncthreads();                                               // every warp has left its ring
   if (*s_abort && warp == W && lane < W)                         // after a failure: the copies in flight
-    for (int i = max(0, issued - NST); i < issued; i++)
-      if (i * W + lane < n) drain_phase(&full[i % NST * W + lane], (uint32_t)(i / NST) & 1u);
+    drain_ring_order<NST>(issued, [&](uint32_t stage, uint32_t parity) { drain_phase(&full[stage * W + lane], parity); });
   __syncthreads();
   float* part = reinterpret_cast<float*>(sm);
   if (warp < W) {

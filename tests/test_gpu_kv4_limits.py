@@ -2,7 +2,9 @@
 import pytest
 import torch
 
-from flint_b200 import _lib
+from flint_b200 import _lib, packing
+from flint_b200.config import ModelArgs
+from flint_b200.engine import DecodeEngine
 from tests.test_gpu_kv4 import check_attention, make, rows
 
 pytestmark = pytest.mark.gpu
@@ -31,3 +33,27 @@ def test_many_rows_leave_out_pages_that_the_table_does_not_have(hd, nkv, missing
         st = c.status()
         assert st["code"] == _lib.FB_ERR_RANGE and st["where"] == 21
         check_attention(out, q, K[seen], V[seen], cached - 64 * len(missing), hd ** -0.5, wide=True)
+
+
+@pytest.mark.parametrize("name,M,pos,limits", [("tiny", 1, 10000, (0, 0, 3, 20, 100, 300)), ("tiny", 3, 10000, (0, 10, 100)), ("llama-8b-class", 1, 32700, (0, 0, 3, 20, 100, 300)),
+                                               ("llama-8b-class", 2, 9000, (0, 20, 300))])
+def test_passes_over_long_caches_that_give_up_leave_nothing_behind(name, M, pos, limits):
+    """Limits of the waits from nothing on, in launches whose copying warp comes back to a stage more than once: the next clean pass gives the bits of the first."""
+    cfg = ModelArgs.from_name(name)
+    if name != "tiny":
+        cfg.n_layer, cfg.vocab_size = 1, 512
+    eng = DecodeEngine(cfg, packing.synth_packed(cfg, 0, device=DEV), max_seq=pos + 64, kv_bits=4)
+    for layer in range(cfg.n_layer):
+        eng.cache.append(layer, rows(2 * layer, pos, cfg.n_local_heads, cfg.head_dim), rows(2 * layer + 1, pos, cfg.n_local_heads, cfg.head_dim), 0)
+    toks = torch.arange(5, 5 + M, dtype=torch.int32, device=DEV)
+    run = (lambda: eng.decode(17, pos).clone()) if M == 1 else (lambda: eng.verify(toks, pos)[0])
+    want = run()
+    eng.check()
+    for limit in limits * 2:
+        eng.set_option(0, limit)
+        run()
+        assert eng.status()["code"] in (_lib.FB_OK, _lib.FB_ERR_TIMEOUT)
+        eng.set_option(0, 4000000)
+        again = run()
+        eng.check()
+        assert torch.equal(want, again)

@@ -1,6 +1,7 @@
 """CPU: what a launch over the 4-bit cache that gives up waits for before it ends (flint_b200/csrc/fb_drain.hpp), run against a model of the barriers in which everything ends
 as late as it can: nothing may be in flight behind it, and no wait may be one that nothing ends."""
 import ctypes
+import itertools
 import os
 import subprocess
 
@@ -11,9 +12,11 @@ SHIM = """
 #include "fb_drain.hpp"
 typedef void (*Wait)(uint32_t);
 typedef void (*Commit)();
+typedef void (*RingWait)(uint32_t, uint32_t);
+extern "C" void ring(uint32_t issued, RingWait wait) { fb::drain_ring_order<3>(issued, wait); }
 extern "C" void commits(uint32_t committed, Wait wait, Commit commit) { fb::drain_commit_order(committed, wait, commit); }
 """
-WAIT, COMMIT = ctypes.CFUNCTYPE(None, ctypes.c_uint32), ctypes.CFUNCTYPE(None)
+WAIT, RING_WAIT, COMMIT = ctypes.CFUNCTYPE(None, ctypes.c_uint32), ctypes.CFUNCTYPE(None, ctypes.c_uint32, ctypes.c_uint32), ctypes.CFUNCTYPE(None)
 
 
 @pytest.fixture(scope="module")
@@ -40,6 +43,34 @@ class Barrier:
     @property
     def quiet(self):
         return self.over == self.armed and not self.hung
+
+
+def ring_of(issued, under_way):
+    """A ring of three stages that copies 0 .. issued-1 went to, stage after stage, those in `under_way` not over."""
+    stages = [Barrier() for _ in range(3)]
+    for i in range(issued):
+        stages[i % 3].armed += 1
+        stages[i % 3].over += i not in under_way
+    return stages
+
+
+@pytest.mark.parametrize("issued", range(11))
+def test_every_copy_has_ended(lib, issued):
+    last = range(max(0, issued - 3), issued)               # the last one of a stage may be under way, those before it are over
+    for under_way in itertools.chain.from_iterable(itertools.combinations(last, n) for n in range(4)):
+        stages = ring_of(issued, under_way)
+        lib.ring(issued, RING_WAIT(lambda s, parity: stages[s].wait(parity)))
+        assert all(b.quiet for b in stages)
+
+
+def test_a_copy_that_was_not_issued_does_not_count(lib):
+    """One too many: the oldest copy is passed over while it is under way, and a wait that nothing ends where it is not."""
+    stages = ring_of(4, {1})
+    lib.ring(5, RING_WAIT(lambda s, parity: stages[s].wait(parity)))
+    assert not stages[1].quiet and not stages[1].hung
+    stages = ring_of(4, set())
+    lib.ring(5, RING_WAIT(lambda s, parity: stages[s].wait(parity)))
+    assert stages[1].hung
 
 
 @pytest.mark.parametrize("committed", range(7))
