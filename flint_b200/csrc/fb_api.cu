@@ -476,6 +476,7 @@ int fb_bind_kv4(fb_ctx* c, const fb_kv4_seqs* s, int64_t layer_bytes, const uint
   c->kv4 = *s;
   c->kv4.d_start = c->kv4.d_cached = nullptr;
   c->kv4.d_status = (int32_t*)c->status;
+  c->kv4.cached = c->kv4.n_tokens = 0;                         // a pass has its own; moves have none
   c->kv4_layer = layer_bytes; c->kv4_freq = d_freq;
   c->max_seq = s->table_ld * 64;
   c->kv4_bound = true;

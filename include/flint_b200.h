@@ -274,8 +274,8 @@ int fb_kv4_compact(const fb_kv4_seqs* seqs, int32_t n_layer, int64_t layer_bytes
 int fb_kv4_move(const fb_kv4_seqs* seqs, int32_t n_layer, int64_t layer_bytes, const int32_t* src, const int32_t* dst, int32_t n, void* stream);
 
 /* A context's cache in 4 bits instead of fb_bind_kv's (the one bound last is used; a tensor-parallel context: FB_ERR_STATE). seqs: pool of n_layer layers
- * layer_bytes apart, one sequence's table, n_pages, table_ld; its other fields are not read and errors go to fb_last_status. d_freq as in fb_kv4_append, for the model's
- * rotation; pool, table and d_freq must stay alive. The M-token passes append to it and attend over it, a decode step is such a pass of one token (fb_decode: the same
+ * layer_bytes apart, one sequence's table, n_pages, table_ld; head_dim and n_kv_head are the model's (else FB_ERR_SHAPE), n_seq is 1 and device the context's (else
+ * FB_ERR_ARG). d_start, d_cached, d_status, cached and n_tokens are not read, errors go to fb_last_status. d_freq as in fb_kv4_append, for the model's rotation; pool, table and d_freq must stay alive. The M-token passes append to it and attend over it, a decode step is such a pass of one token (fb_decode: the same
  * arguments and results), fb_kv_move and fb_kv_compact move its rows. */
 int fb_bind_kv4(fb_ctx* ctx, const fb_kv4_seqs* seqs, int64_t layer_bytes, const uint64_t* d_freq);
 

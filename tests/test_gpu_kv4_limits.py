@@ -1,11 +1,13 @@
 """GPU: the 4-bit cache where its calls can go wrong: pages that the table does not have, rows that nobody sees, numbers of every size, sequences that cannot be."""
+import ctypes
+
 import pytest
 import torch
 
 from flint_b200 import _lib, packing
 from flint_b200.config import ModelArgs
 from flint_b200.engine import DecodeEngine
-from tests.test_gpu_kv4 import check_attention, make, rows
+from tests.test_gpu_kv4 import check_attention, ints, make, rows
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -57,3 +59,26 @@ def test_passes_over_long_caches_that_give_up_leave_nothing_behind(name, M, pos,
         again = run()
         eng.check()
         assert torch.equal(want, again)
+
+
+def test_a_bound_cache_takes_nothing_from_the_fields_that_are_not_read():
+    """The structure of some earlier call, its lengths those of that call."""
+    cfg = ModelArgs.from_name("tiny")
+    packed = packing.synth_packed(cfg, 0, device=DEV)
+    got = []
+    for cached, n_tokens in ((0, 0), (1000, 128), (-7, -9), (128, 2 ** 31 - 1)):
+        eng = DecodeEngine(cfg, packed, max_seq=128, kv_bits=4)
+        s = eng.cache._one(0, 0)
+        s.cached, s.n_tokens, s.d_start, s.d_cached, s.d_status = cached, n_tokens, 4096, 4096, None
+        _lib.check(eng.lib.fb_bind_kv4(eng._ctx, ctypes.byref(s), eng.cache.layer_bytes, eng.cache.freq.data_ptr()), "fb_bind_kv4")
+        toks = torch.arange(5, 25, dtype=torch.int32, device=DEV)
+        eng.prefill(toks, 0)
+        eng.kv_move([3, 4, 100], [5, 3, 127])
+        eng.kv_compact(ints(3, 0, 0, 2, 6), 10)
+        got.append(eng.decode(17, 20).clone())
+        eng.check()
+        assert torch.equal(got[0], got[-1])
+        for name in ("head_dim", "n_kv_head", "n_seq", "device"):
+            t = eng.cache._one(0, 0)
+            setattr(t, name, getattr(t, name) + 1)
+            assert eng.lib.fb_bind_kv4(eng._ctx, ctypes.byref(t), eng.cache.layer_bytes, eng.cache.freq.data_ptr()) in (_lib.FB_ERR_SHAPE, _lib.FB_ERR_ARG)
