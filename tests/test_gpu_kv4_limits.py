@@ -7,7 +7,8 @@ import torch
 from flint_b200 import _lib, packing
 from flint_b200.config import ModelArgs
 from flint_b200.engine import DecodeEngine
-from tests.test_gpu_kv4 import check_attention, ints, make, rows
+from tests import kv4_bounds
+from tests.test_gpu_kv4 import check_attention, filled, gen, ints, make, rows
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -82,3 +83,42 @@ def test_a_bound_cache_takes_nothing_from_the_fields_that_are_not_read():
             t = eng.cache._one(0, 0)
             setattr(t, name, getattr(t, name) + 1)
             assert eng.lib.fb_bind_kv4(eng._ctx, ctypes.byref(t), eng.cache.layer_bytes, eng.cache.freq.data_ptr()) in (_lib.FB_ERR_SHAPE, _lib.FB_ERR_ARG)
+
+
+# ---------------------------------------------------------------------------------------------------------------- what comes out, as near as the roundings let it
+@pytest.mark.parametrize("hd,nh,nkv", [(64, 40, 8), (80, 32, 8), (128, 32, 8), (64, 9, 1), (128, 34, 2)])
+@pytest.mark.parametrize("cached,new,qscale", [(0, 1, 1.5), (31, 2, 1.5), (200, 1, 1.5), (1344, 3, 1.0), (1345, 1, 1.0), (5000, 1, 1.0), (11000, 1, 0.5), (33000, 1, 0.3), (33000, 3, 3.0)])
+def test_few_rows_within_their_roundings(hd, nh, nkv, cached, new, qscale):
+    """One CTA a group of rows, clusters, parts that a second launch joins. Flat scores: every page weighs."""
+    c, K, V, q, _ = filled([cached], [new], nh, nkv, hd, seed=cached + hd, qscale=qscale)
+    out = c.attend(0, q, cached)
+    c.check()
+    kv4_bounds.check(out, *kv4_bounds.bounds(q, K[0], V[0], cached, hd ** -0.5))
+
+
+@pytest.mark.parametrize("hd,nh,nkv", [(64, 40, 8), (80, 32, 8), (128, 32, 8), (128, 8, 2)])
+@pytest.mark.parametrize("cached,new,qscale", [(0, 70, 1.5), (0, 300, 1.5), (1000, 26, 1.5), (3001, 61, 1.0), (129, 200, 1.5), (9000, 33, 0.3)])
+def test_many_rows_within_their_roundings(hd, nh, nkv, cached, new, qscale):
+    c, K, V, q, _ = filled([cached], [new], nh, nkv, hd, seed=cached + hd, qscale=qscale)
+    out = c.attend(0, q, cached)
+    c.check()
+    kv4_bounds.check(out, *kv4_bounds.bounds(q, K[0], V[0], cached, hd ** -0.5, many=new * nh // nkv > 64))
+
+
+@pytest.mark.parametrize("hd,nh,nkv", [(64, 40, 8), (128, 8, 2)])
+@pytest.mark.parametrize("lens,new", [([5, 300, 0, 64, 1, 2000], [1, 1, 0, 1, 1, 1]), ([0, 65, 700], [3, 0, 5]), ([10, 0, 130, 900], [80, 64, 1, 30]), ([3000] * 5, [1] * 5), ([6000, 5, 6000], [2, 2, 1])])
+@pytest.mark.parametrize("masked", [False, True])
+def test_batches_within_their_roundings(hd, nh, nkv, lens, new, masked):
+    """Ragged sequences, causal and each token with a mask of its own over its sequence's new tokens, rows that see nothing of them included."""
+    c, K, V, q, start = filled(lens, new, nh, nkv, hd, seed=hd)
+    amask = None
+    if masked:
+        amask = (torch.rand(sum(new), max(new) + 3, generator=gen(7), device=DEV) < 0.5).to(torch.uint8)
+        amask[::3] = 0
+    many = max(new) * nh // nkv > 64
+    out = c.attend(0, q, ints(*lens), start=start, amask=amask, max_new=max(new))
+    c.check()
+    for b in range(len(lens)):
+        a, z = int(start[b]), int(start[b + 1])
+        if z > a:
+            kv4_bounds.check(out[a:z], *kv4_bounds.bounds(q[a:z], K[b], V[b], lens[b], hd ** -0.5, None if amask is None else amask[a:z], many=many))
