@@ -6,7 +6,7 @@
 // tiles take turns: one multiplies while the other exponentiates. Keys and values are dequantised once for both tiles by six warps into the K-major
 // 128-byte-swizzle layout that the MMA reads, K as [position][dim], V as [dim][position], each number (nib - 8) s + z rounded once. (Operands nib - 8, with s and z in the
 // softmax as kv4_attn_few has them, would be exact, but cost the softmax, which is what bounds this kernel, twice its instructions.) All operands are fp16, half a step
-// 2^-11: K times a power of two per step (2^-25 of the largest key of its 128 positions at the smallest), Q times one per row, P times 2^7, V as it is. A page whose
+// 2^-11: K times a power of two per step (per position where the keys of its 128 positions are more than 2^23 apart), Q times one per row, P times 2^7, V as it is. A page whose
 // rows of V have bounds 8 |s| + |z| outside [2^-10, 2^15) has its V and P in bf16, half a step 2^-8: there rows of any size stand side by side, whatever their weight.
 // (With bf16 operands throughout 1000 tokens of 32 heads of 128 behind 7011 took 152 us, but outputs were off by 0.0044 of their 2-norm; now 166 us, 743 TFLOP/s, and 0.0017,
 // which is the rounding of the output itself. What is dearer is the factors' look and conversion, and P's second form. Tried and slower: factors converted in place by the
@@ -30,7 +30,7 @@ struct Kv4Many {
   static constexpr int ND = 4;                                              // steps whose notes are kept: softmax may be at i when step i + 2 is dequantised
   static constexpr int NR = 4;                                              // pages: two being dequantised, two on their way
   static constexpr int Q = 0, K = Q + 2 * QT, V = K + 2 * KT, RAW = V + 4 * VT, BAR = RAW + NR * REC;
-  static constexpr int BARS = 2 * NR + 17, TOTAL = BAR + BARS * 8 + 2 * ND * 8 + (2 + 2 + NR + 2 * ND) * 4;       // barriers, then what stands behind them in the kernel
+  static constexpr int BARS = 2 * NR + 17, TOTAL = BAR + BARS * 8 + 2 * ND * 8 + (2 + 2 + NR + 2 * ND) * 4 + ND * kManyStep;       // barriers, then what stands behind them in the kernel
   static constexpr int T_S = 0, T_O = 256, TCOLS = 512;                     // tensor memory columns: two S / P, two O
   static_assert(TOTAL <= 227 * 1024 && T_O + 2 * HD <= TCOLS && QT % 1024 == 0 && VT % 1024 == 0 && RAW % 16 == 0 && REC % 16 == 0, "plan");
 };
@@ -103,8 +103,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   volatile int* s_issued = s_abort + 1;                          // [2] pages, PV of tile 0
   volatile int* s_none = s_issued + 2;                           // [NR] the page does not exist
-  volatile int* s_gone = s_none + NR;                            // [ND steps] bit p: page p of the step does not exist, bit 2 + p: it is wide
+  volatile int* s_gone = s_none + NR;                            // [ND steps] bit p: page p of the step does not exist, bit 2 + p: it is wide, bit 4: keys have powers of two of their own
   volatile float* s_kscale = reinterpret_cast<volatile float*>(s_gone + M::ND);  // [ND steps] inverse of the power of two of the keys
+  uint8_t* s_kown = reinterpret_cast<uint8_t*>(const_cast<float*>(s_kscale + M::ND));      // [ND steps][positions] bit 4: its exponent
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Kv4Seqs& S = P.S;
   pdl_begin(true);
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
     const int dw = warp - 8;
     constexpr int QN = C::MAIN / 32, PT = 32 / QN, KTURNS = kPage / PT, VTURNS = C::MAIN / 16;       // lanes of a position, positions of a turn, turns of a page
     float kf = 1.f;                                              // the step's power of two of the keys
-    auto key = [&](const uint8_t* rec, uint8_t* kt, int p, int w0, auto words) {           // words w0 .. of position p
+    auto key = [&](const uint8_t* rec, uint8_t* kt, int p, int w0, auto words, auto apart, uint8_t* own) {           // words w0 .. of position p
       constexpr int NWD = decltype(words)::value;
       const uint8_t* blk = rec + (p >> 4) * C::BLOCK;
       uint32_t x[NWD];
@@ -241,7 +242,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
         x[0] = w.x; x[1] = w.y;
       }
       const uint32_t sz = *reinterpret_cast<const uint32_t*>(blk + C::KSZ + (p & 15) * 4);
-      const uint32_t f = cvt_f16x2(bflo(sz) * kf, bfhi(sz) * kf);
+      float by = kf;
+      if (decltype(apart)::value) {                              // a power of two of the position's own
+        const float2 f = pow2_for(fmaf(8.f, fabsf(bflo(sz)), fabsf(bfhi(sz))));
+        by = f.x;
+        if (w0 == 0) own[p] = (uint8_t)(__float_as_uint(f.y) >> 23);
+      }
+      const uint32_t f = cvt_f16x2(bflo(sz) * by, bfhi(sz) * by);
       const __half2 s = kv4_h2(__byte_perm(f, f, 0x1010)), z = kv4_h2(__byte_perm(f, f, 0x3232));
       uint8_t* row = kt + (w0 >> 3) * (kManyStep * 128) + p * 128;
 #pragma unroll
@@ -298,8 +305,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       const int left0 = total - (task.unit + i) * kManyStep, left1 = left0 - kPage;                // positions of the pages that exist
       const bool none0 = s_none[r] != 0, none1 = s_none[r + 1] != 0 || left1 <= 0;
       // Positions whose V is NaN: those, and what lies behind the last position, become zeros, as every row of P multiplies them. A page whose rows of V
-      // have bounds 8 |s| + |z| (its largest value that there can be) beyond [2^-10, 2^15) is `wide`; kmost: the largest bound of a key.
-      uint32_t kmost = 0;
+      // have bounds 8 |s| + |z| (its largest value that there can be) beyond [2^-10, 2^15) is `wide`; kmost, kleast: the largest bound of a key, the smallest but 0.
+      uint32_t kmost = 0, kleast = 0x7f800000u;
       bool wide0 = false, wide1 = false;
       auto look = [&](const uint8_t* rec, int left, bool& wide) {
         uint32_t bad[2];
@@ -309,31 +316,40 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
           const uint32_t a = *reinterpret_cast<const uint32_t*>(at + C::KSZ), c = *reinterpret_cast<const uint32_t*>(at + C::VSZ);
           const bool in = 32 * k + lane < left, num = bflo(c) < INFINITY;
           const float kb = fmaf(8.f, fabsf(bflo(a)), fabsf(bfhi(a))), vb = fmaf(8.f, fabsf(bflo(c)), fabsf(bfhi(c)));
-          if (in && kb < INFINITY) kmost = max(kmost, __float_as_uint(kb));
+          if (in && kb < INFINITY) {
+            kmost = max(kmost, __float_as_uint(kb));
+            if (kb > 0.f) kleast = min(kleast, __float_as_uint(kb));
+          }
           bad[k] = __ballot_sync(0xffffffffu, in && !num);
           wide |= __any_sync(0xffffffffu, in && num && vb != 0.f && !(vb >= 0x1p-10f && vb < 0x1p15f)) != 0;
         }
         return (unsigned long long)bad[0] | (unsigned long long)bad[1] << 32;
       };
-      // The usual case at a glance: whole pages, all factors within narrower bounds than that: s of V from 2^-13 to below 2^11, |z| below 2^14, no NaN and no infinity of K.
+      // The usual case at a glance: whole pages, all factors within narrower bounds than that: s of V from 2^-13 to below 2^11, |z| below 2^14, of K s from 2^-12 on and
+      // the same above.
       unsigned long long bad0 = 0, bad1 = 0;
+      bool apart = false;
       {
         const uint8_t* at = rec0 + (lane >> 4) * C::BLOCK + (lane & 15) * 4;
-        uint32_t km = 0, vm = 0, vs = 0xffffu;
+        uint32_t km = 0, vm = 0, ks = 0xffffu, vs = 0xffffu;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           const uint32_t a = *reinterpret_cast<const uint32_t*>(at + (k >> 1) * REC + 2 * (k & 1) * C::BLOCK + C::KSZ) & 0x7fff7fffu,
                          c = *reinterpret_cast<const uint32_t*>(at + (k >> 1) * REC + 2 * (k & 1) * C::BLOCK + C::VSZ) & 0x7fff7fffu;
           km = __vmaxu2(km, a);
           vm = __vmaxu2(vm, c);
+          ks = min(ks, a & 0xffffu);
           vs = min(vs, c & 0xffffu);
         }
-        const bool usual = __vmaxu2(km, 0x7e007e00u) == 0x7e007e00u && __vmaxu2(vm, 0x467f44ffu) == 0x467f44ffu && vs >= 0x3900u;
+        const bool usual = __vmaxu2(__vmaxu2(km, vm), 0x467f44ffu) == 0x467f44ffu && vs >= 0x3900u && ks >= 0x3980u;
         if (__all_sync(0xffffffffu, usual) && !none0 && !none1 && left1 >= kPage) {
           kmost = __float_as_uint(fmaf(8.f, bflo(km), bfhi(km)));
         } else {
           if (!none0) bad0 = look(rec0, left0, wide0);
           if (!none1) bad1 = look(rec1, left1, wide1);
+          // One power of two does for keys whose bounds are 2^24 apart or less (fp16 then holds them from 2^-10 on); beyond that each has its own, so that a key
+          // that is not seen, or as nothing to the softmax, takes no bits from the others.
+          apart = (int)(__reduce_max_sync(0xffffffffu, kmost) >> 23) - (int)(__reduce_min_sync(0xffffffffu, kleast) >> 23) > 23;
         }
       }
       const float2 kp = pow2_for(__uint_as_float(__reduce_max_sync(0xffffffffu, kmost)));          // the largest into [2^14, 2^15)
@@ -344,21 +360,27 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
         const int note = i & (M::ND - 1);
         s_bad[2 * note] = bad0;
         s_bad[2 * note + 1] = bad1;
-        s_gone[note] = (none0 ? 1 : 0) | (none1 ? 2 : 0) | (wide0 ? 4 : 0) | (wide1 ? 8 : 0);
-        s_kscale[note] = kp.y;
+        s_gone[note] = (none0 ? 1 : 0) | (none1 ? 2 : 0) | (wide0 ? 4 : 0) | (wide1 ? 8 : 0) | (apart ? 16 : 0);
+        s_kscale[note] = apart ? 1.f : kp.y;
       }
-      if (!none0 && !none1) {
+      if (!none0 && !none1 && !apart) {
 #pragma unroll 1
         for (int it = dw; it < 2 * KTURNS; it += kManyDequant) {
           const int h = it / KTURNS, j = it % KTURNS;
-          key(h ? rec1 : rec0, kt + h * (kPage * 128), j * PT + lane / QN, 4 * (lane & (QN - 1)), four);
+          key(h ? rec1 : rec0, kt + h * (kPage * 128), j * PT + lane / QN, 4 * (lane & (QN - 1)), four, std::false_type(), nullptr);
         }
-        if (HD == 80 && dw >= 2) key(dw < 4 ? rec0 : rec1, kt + (dw < 4 ? 0 : kPage * 128), (dw & 1) * 32 + lane, 8, two);
+        if (HD == 80 && dw >= 2) key(dw < 4 ? rec0 : rec1, kt + (dw < 4 ? 0 : kPage * 128), (dw & 1) * 32 + lane, 8, two, std::false_type(), nullptr);
       } else {
+        auto page = [&](int h, auto a) {
+          uint8_t* own = s_kown + (i & (M::ND - 1)) * kManyStep + h * kPage;
+#pragma unroll 1
+          for (int j = dw; j < KTURNS; j += kManyDequant) key(h ? rec1 : rec0, kt + h * (kPage * 128), j * PT + lane / QN, 4 * (lane & (QN - 1)), four, a, own);
+          if (HD == 80 && dw < 2) key(h ? rec1 : rec0, kt + h * (kPage * 128), dw * 32 + lane, 8, two, a, own);
+        };
         for (int h = 0; h < 2; h++) {
           if (h ? none1 : none0) continue;
-          for (int j = dw; j < KTURNS; j += kManyDequant) key(h ? rec1 : rec0, kt + h * (kPage * 128), j * PT + lane / QN, 4 * (lane & (QN - 1)), four);
-          if (HD == 80 && dw < 2) key(h ? rec1 : rec0, kt + h * (kPage * 128), dw * 32 + lane, 8, two);
+          if (apart) page(h, std::true_type());
+          else page(h, std::false_type());
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -439,7 +461,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       const float c2 = fmaxf(cs * s_kscale[note], 1.2e-38f);     // not zero: a score that is not seen stays -inf
       const unsigned long long bad0 = s_bad[2 * note], bad1 = s_bad[2 * note + 1];
       tc_ld_wait();
-      if (p0 + kManyStep > (mask ? seq.cached : min(total, seq.cached + m_first + 1)) || (gone & 3) || (bad0 | bad1)) {
+      if (p0 + kManyStep > (mask ? seq.cached : min(total, seq.cached + m_first + 1)) || (gone & 19) || (bad0 | bad1)) {
+        if (gone & 16) {
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int e = 0; e < 32; e++) v[c][e] = __float_as_uint(__uint_as_float(v[c][e]) * __uint_as_float((uint32_t)s_kown[note * kManyStep + c * 32 + e] << 23));
+        }
         // what is not seen becomes -inf
         uint32_t vis[4];
 #pragma unroll

@@ -122,3 +122,45 @@ def test_batches_within_their_roundings(hd, nh, nkv, lens, new, masked):
         a, z = int(start[b]), int(start[b + 1])
         if z > a:
             kv4_bounds.check(out[a:z], *kv4_bounds.bounds(q[a:z], K[b], V[b], lens[b], hd ** -0.5, None if amask is None else amask[a:z], many=many))
+
+
+# ---------------------------------------------------------------------------------------------------------------- numbers of every size
+@pytest.mark.parametrize("hd", [64, 80, 128])
+@pytest.mark.parametrize("new", [9, 100])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("power", [20, 30, 60, 100, -30, -90])
+def test_keys_that_a_token_does_not_see_leave_it_alone(hd, new, masked, power):
+    """A new token's key 2^power times the others': tokens ahead of it, or whose masks leave it out, come out within their roundings."""
+    nh, nkv, cached = 8, 2, 100
+    at = new // 2
+    k, v = rows(71, cached + new, nkv, hd), rows(72, cached + new, nkv, hd)
+    k[cached + at] = (k[cached + at].float() * 2.0 ** power).bfloat16()
+    c = make([cached + new], nkv, hd, base=None, garbage=True)
+    c.append(0, k, v, 0)
+    K, V = c.read(0, cached + new, 0)
+    q = rows(73, new, nh, hd, 1.5)
+    amask = torch.ones(new, new, dtype=torch.uint8, device=DEV).tril() if masked else None
+    if masked:
+        amask[:, at] = 0
+    out = c.attend(0, q, cached, amask=amask)
+    c.check()
+    blind = slice(0, new if masked else at)
+    want = kv4_bounds.bounds(q, K, V, cached, hd ** -0.5, amask, many=new * nh // nkv > 64)
+    kv4_bounds.check(out[blind], *(x[blind] for x in want))
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_keys_of_many_sizes_side_by_side(new):
+    """Keys from 2^-60 to 2^60 of the usual size, positions in random order; a query per size, 2^-60 to 2^60 times the usual, so that some keys decide and others are as nothing."""
+    hd, nkv, nh, cached = 64, 1, 4, 400
+    n = cached + new
+    g = gen(80)
+    size = torch.randint(-60, 1, (n,), generator=g, device=DEV).double().exp2().float()
+    k = (torch.randn(n, nkv, hd, generator=g, device=DEV).abs() * size[:, None, None]).bfloat16()
+    q = (-torch.randn(new, nh, hd, generator=g, device=DEV).abs() * torch.tensor([1.0, 2.0 ** 20, 2.0 ** 40, 2.0 ** 60], device=DEV)[:, None]).bfloat16()
+    c = make([n], nkv, hd, base=None, garbage=True)
+    c.append(0, k, rows(81, n, nkv, hd), 0)
+    K, V = c.read(0, n, 0)
+    out = c.attend(0, q, cached)
+    c.check()
+    kv4_bounds.check(out, *kv4_bounds.bounds(q, K, V, cached, hd ** -0.5, many=new * nh > 64))
