@@ -358,6 +358,7 @@ __device__ __forceinline__ uint32_t cvt_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
+constexpr float kLowest = -3.402823466e38f;        // a row's running maximum before any score: finite, so that differences from it are numbers, and below every score but -inf
 struct Kv4Attend {
   Kv4Seqs S;
   const uint16_t* q;         // bf16 [T][nh][HD], rotated, tokens q_ld elements apart
@@ -474,7 +475,7 @@ struct Kv4Task {
 // Partials of a row, n of them `stride` floats apart, eight loads side by side: lane < HD / 4 merges dims 4 lane .. 4 lane + 3
 template <int HD>
 __device__ __forceinline__ void kv4_merge(const float* p0, int n, size_t stride, int lane, float4& acc, float& mm, float& den) {
-  mm = -1e30f;
+  mm = kLowest;
   den = 0.f;
   acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
@@ -648,7 +649,7 @@ __global__ void __launch_bounds__(W * 32 + 32) kv4_attn_few(const Kv4Attend P) {
     for (int i = 0; i < MT; i++) o[nq][i][0] = o[nq][i][1] = o[nq][i][2] = o[nq][i][3] = 0.f;
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-      mrun[nq][e] = -1e30f; lrun[nq][e] = 0.f; zrun[nq][e] = 0.f;
+      mrun[nq][e] = kLowest; lrun[nq][e] = 0.f; zrun[nq][e] = 0.f;
       wtop[nq][e] = 0.f; wlim[nq][e] = 0.f; vf[nq][e] = 1.f; erun[nq][e] = 127;
     }
   }
@@ -743,7 +744,7 @@ __global__ void __launch_bounds__(W * 32 + 32) kv4_attn_few(const Kv4Attend P) {
           float mx = -INFINITY;
 #pragma unroll
           for (int k = 0; k < U / 16; k++) mx = fmaxf(mx, fmaxf(sc[nq][k][e], sc[nq][k][2 + e]));
-          const float mn = fmaxf(mrun[nq][e], top(mx));          // finite from below: the running maximum starts at -1e30
+          const float mn = fmaxf(mrun[nq][e], top(mx));          // finite from below
           cr[e] = ex2(mrun[nq][e] - mn);
           mrun[nq][e] = mn;
           lrun[nq][e] *= cr[e]; zrun[nq][e] *= cr[e]; wtop[nq][e] *= cr[e];

@@ -328,7 +328,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       // The usual case at a glance: whole pages, all factors within narrower bounds than that: s of V from 2^-13 to below 2^11, |z| below 2^14, of K s from 2^-12 on and
       // the same above.
       unsigned long long bad0 = 0, bad1 = 0;
-      bool apart = false;
       {
         const uint8_t* at = rec0 + (lane >> 4) * C::BLOCK + (lane & 15) * 4;
         uint32_t km = 0, vm = 0, ks = 0xffffu, vs = 0xffffu;
@@ -347,12 +346,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
         } else {
           if (!none0) bad0 = look(rec0, left0, wide0);
           if (!none1) bad1 = look(rec1, left1, wide1);
-          // One power of two does for keys whose bounds are 2^24 apart or less (fp16 then holds them from 2^-10 on); beyond that each has its own, so that a key
-          // that is not seen, or as nothing to the softmax, takes no bits from the others.
-          apart = (int)(__reduce_max_sync(0xffffffffu, kmost) >> 23) - (int)(__reduce_min_sync(0xffffffffu, kleast) >> 23) > 23;
         }
       }
-      const float2 kp = pow2_for(__uint_as_float(__reduce_max_sync(0xffffffffu, kmost)));          // the largest into [2^14, 2^15)
+      // One power of two does for keys whose bounds are 2^24 apart or less (fp16 then holds them from 2^-10 on); beyond that each has its own, so that a key
+      // that is not seen, or as nothing to the softmax, takes no bits from the others.
+      const uint32_t kmax = __reduce_max_sync(0xffffffffu, kmost);
+      const bool apart = __any_sync(0xffffffffu, (kmax >> 23) > (kleast >> 23) + 23u);
+      const float2 kp = pow2_for(__uint_as_float(kmax));         // the largest into [2^14, 2^15)
       kf = kp.x;
       const bool special = none0 || none1 || bad0 || bad1 || left1 < kPage || wide0 || wide1;
       if (dw == 0 && lane == 0) {
@@ -449,7 +449,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
     }
     const uint8_t* mask = P.amask ? P.amask + (size_t)(seq.first + mq) * P.mask_ld : nullptr;
     const int m_first = (task.r0 + min(t * 128 + (warp & 3) * 32, rows - 1)) / R;          // the warp's first token: what it sees, all rows see
-    float m = -1e30f, l = 0.f;
+    float m = kLowest, l = 0.f;
+    // Exponents are a score's product with c2, not rounded, less m, which was: by less than half a power of two below 2^22. From there on products are rounded first.
+    bool large = false;
+    int plain = mask ? seq.cached : min(total, seq.cached + m_first + 1);                 // steps that end here or before need no look at what is seen; large: none
     for (int i = 0; i < n; i++) {
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], (uint32_t)i & 1u, wc, W_FULL, 50));
       if (!ok) break;
@@ -458,15 +461,22 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
 #pragma unroll
       for (int c = 0; c < 4; c++) tc_ld32(ts + c * 32, v[c]);
       const int p0 = (task.unit + i) * kManyStep, note = i & (M::ND - 1), gone = s_gone[note];
-      const float c2 = fmaxf(cs * s_kscale[note], 1.2e-38f);     // not zero: a score that is not seen stays -inf
+      float c2 = fmaxf(cs * s_kscale[note], 1.2e-38f);           // not zero: a score that is not seen stays -inf
       const unsigned long long bad0 = s_bad[2 * note], bad1 = s_bad[2 * note + 1];
       tc_ld_wait();
-      if (p0 + kManyStep > (mask ? seq.cached : min(total, seq.cached + m_first + 1)) || (gone & 19) || (bad0 | bad1)) {
-        if (gone & 16) {
+      if (p0 + kManyStep > plain || (gone & 19) || (bad0 | bad1)) {
+        if (__builtin_expect(gone & 16, 0)) {
 #pragma unroll
           for (int c = 0; c < 4; c++)
 #pragma unroll
             for (int e = 0; e < 32; e++) v[c][e] = __float_as_uint(__uint_as_float(v[c][e]) * __uint_as_float((uint32_t)s_kown[note * kManyStep + c * 32 + e] << 23));
+        }
+        if (__builtin_expect(large, 0)) {
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int e = 0; e < 32; e++) v[c][e] = __float_as_uint(__uint_as_float(v[c][e]) * c2);
+          c2 = 1.f;
         }
         // what is not seen becomes -inf
         uint32_t vis[4];
@@ -498,6 +508,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       const float top = fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[4]), max3(mx[5], mx[6], mx[7])) * c2;
       if (__any_sync(0xffffffffu, top > m + 8.f)) {
         const float mn = fmaxf(m, top), corr = ex2(m - mn);
+        if (!large && __any_sync(0xffffffffu, fabsf(mn) >= 0x1p22f && mn > kLowest)) {
+          large = true;                                          // the step once more
+          plain = 0;
+          i--;
+          continue;
+        }
         if (i > 0) {                                             // O as the steps before left it
           ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (uint32_t)(i - 1) & 1u, wc, W_FULL, 51));
           if (!ok) break;

@@ -164,3 +164,36 @@ def test_keys_of_many_sizes_side_by_side(new):
     out = c.attend(0, q, cached)
     c.check()
     kv4_bounds.check(out, *kv4_bounds.bounds(q, K, V, cached, hd ** -0.5, many=new * nh > 64))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,cached", [(1, 0), (1, 300), (2, 9000), (1, 40000), (40, 0), (40, 300), (130, 2000)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("power", [12, 22, 25, 28, 40, 98, 108])
+def test_scores_of_any_size(hd, new, cached, sign, power):
+    """All keys lie along one direction, the queries too, 2^power long; one position of the first 30 is ahead of all others by a sixth of its score or more (far more than a
+    rounding): it takes everything, also where all scores are far below zero. Flat keys: equal scores of that size share evenly."""
+    nh, nkv, n = 8, 2, cached + new
+    g = gen(90)
+    u = (torch.rand(hd, generator=g, device=DEV) + 0.5).bfloat16().float()
+    a = torch.rand(n, 1, 1, generator=g, device=DEV) * 0.4 + 0.6
+    first = min(n, 30) // 3
+    a[first] = 1.2 if sign > 0 else 0.45
+    c = make([n], nkv, hd, base=None, garbage=True)
+    c.append(0, (a * u).expand(n, nkv, hd).bfloat16(), rows(91, n, nkv, hd), 0)
+    _, V = c.read(0, n, 0)
+    q = (u * sign * 2.0 ** power).expand(new, nh, hd).bfloat16()
+    out = c.attend(0, q, cached)
+    c.check()
+    sees = slice(max(0, first - cached), new)
+    want = V[first].repeat_interleave(nh // nkv, 0).expand(new, nh, hd)
+    # the output to bf16; probability or probability times s, and the value, to fp16
+    tol = want.abs() * 2.0 ** -8 + 2.0 ** -10 * V.abs().amax()
+    assert ((out - want).abs() <= tol)[sees].all()
+    if n <= 400:
+        c.append(0, torch.ones(n, nkv, hd, dtype=torch.bfloat16, device=DEV), rows(92, n, nkv, hd), 0)
+        _, V = c.read(0, n, 0)
+        out = c.attend(0, q, cached)
+        c.check()
+        want = (V.double().cumsum(0) / torch.arange(1, n + 1, device=DEV)[:, None, None]).repeat_interleave(nh // nkv, 1)[cached:]
+        assert ((out - want).abs() <= want.abs() * 2.0 ** -8 + 2.0 ** -10 * V.abs().amax()).all()
