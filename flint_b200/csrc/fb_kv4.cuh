@@ -80,11 +80,22 @@ template <int HD>
 __device__ __forceinline__ uint8_t* kv4_block(const Kv4Seqs& S, int page, int head, int slot) {
   return S.pool + ((size_t)page * S.nkv + head) * Kv4<HD>::REC + (slot % kPage / 16) * Kv4<HD>::BLOCK;
 }
-// The sequence of token m, found by a whole warp: how many sequences end at or before it. -1: behind the last one.
-__device__ __forceinline__ int kv4_seq_of(const Kv4Seqs& S, int m, int lane) {
+// Does sequence b end ahead of its start? Then nothing of the call is done: tokens could be two sequences', and the tasks more than the grid and the scratch have room for.
+__device__ __forceinline__ bool kv4_backward(const Kv4Seqs& S, int b, bool report) {
+  const int first = S.start[b], end = S.start[b + 1];
+  if (end < first && report) kv4_report(S.status, KV4_TOKENS, b, first, end);
+  return end < first;
+}
+// The sequence of token m, found by a whole warp: how many sequences end at or before it. -1: behind the last one, or no call that can be.
+__device__ __forceinline__ int kv4_seq_of(const Kv4Seqs& S, int m, int lane, bool report) {
   if (!S.start) return 0;
   int b = 0;
-  for (int i = 0; i < S.n_seq; i += 32) b += __popc(__ballot_sync(0xffffffffu, i + lane < S.n_seq && S.start[i + lane + 1] <= m));
+  for (int i = 0; i < S.n_seq; i += 32) {
+    const bool in = i + lane < S.n_seq;
+    const unsigned n = __reduce_add_sync(0xffffffffu, in ? (S.start[i + lane + 1] <= m) | (unsigned)kv4_backward(S, i + lane, report) << 8 : 0u);
+    if (n >> 8) return -1;
+    b += (int)n;
+  }
   return b < S.n_seq ? b : -1;
 }
 
@@ -148,7 +159,7 @@ __global__ void __launch_bounds__(256) kv4_append(const Kv4Append P) {
   };
   const int step = gridDim.y * 8;
   uint2 w = load(blockIdx.y * 8 + warp);
-  const int b = kv4_seq_of(S, m, lane);
+  const int b = kv4_seq_of(S, m, lane, m == 0 && blockIdx.y == 0 && warp == 0);
   if (b < 0) return;
   Kv4Seq q;
   const bool first = blockIdx.y == 0 && tid == 0;
@@ -221,7 +232,7 @@ __global__ void __launch_bounds__(256) kv4_read(const Kv4Read P) {
   const Kv4Seqs& S = P.S;
   const int m = blockIdx.x, lane = threadIdx.x & 31;
   pdl_begin(true);
-  const int b = kv4_seq_of(S, m, lane);
+  const int b = kv4_seq_of(S, m, lane, m == 0 && threadIdx.x < 32);
   Kv4Seq q;
   int page = -1, slot = 0;
   if (b >= 0 && q.get(S, b, threadIdx.x == 0) && m >= q.first && m < q.first + q.n) {
@@ -417,10 +428,13 @@ struct Kv4Task {
       }
     } else {
       long long units = 0;
+      bool backward = false;
       for (int i = lane; i < S.n_seq; i += 32) {
         Kv4Seq q;
+        backward = backward || kv4_backward(S, i, report);
         if (q.get(S, i, report)) units += (long long)groups_of(P, q) * units_of(q);
       }
+      if (__any_sync(0xffffffffu, backward)) return false;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
       per = per_of(P, units);

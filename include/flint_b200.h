@@ -237,7 +237,7 @@ int fb_gemv_static(const void* d_q, const void* d_s, const void* d_z, int32_t ro
  *   d_pool    : one layer (fb_kv4_read / compact / move: the first of n_layer layers, layer_bytes apart)
  *   d_table   : device int32 [n_seq][table_ld], page of positions 64 i .. 64 i + 63
  *   d_start   : device int32 [n_seq + 1], tokens d_start[b] .. d_start[b+1] - 1 of the n_tokens are sequence b's; NULL: one sequence has them all. Tokens
- *               behind the last sequence are left alone
+ *               behind the last sequence are left alone. A sequence outside the n_tokens is left out; where d_start[b+1] < d_start[b] for some b, the whole call is
  *   d_cached  : device int32 [n_seq], positions cached ahead of the new tokens; NULL: `cached` for all. New token i of a sequence has slot cached + i
  *   d_status  : device int32[8], zeroed once: word 0 becomes FB_ERR_RANGE when a page, a length or a path in device memory cannot be (what it concerns is
  *               left out, nothing outside the buffers is touched), FB_ERR_TIMEOUT when a bounded wait ran out

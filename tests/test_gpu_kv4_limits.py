@@ -197,3 +197,32 @@ def test_scores_of_any_size(hd, new, cached, sign, power):
         c.check()
         want = (V.double().cumsum(0) / torch.arange(1, n + 1, device=DEV)[:, None, None]).repeat_interleave(nh // nkv, 1)[cached:]
         assert ((out - want).abs() <= want.abs() * 2.0 ** -8 + 2.0 ** -10 * V.abs().amax()).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------- sequences that cannot be
+@pytest.mark.parametrize("T", [3, 142])
+@pytest.mark.parametrize("order", ["0T0T", "0T0", "00T0T", "T0T"])
+def test_starts_that_go_down_leave_out_the_whole_call(T, order):
+    """Two sequences would have the same tokens: nothing is written, no row of another sequence either, and the call is reported."""
+    hd, nkv, nh = 64, 2, 8
+    begin = [T if x == "T" else 0 for x in order]
+    n_seq = len(begin) - 1
+    c = make([T + 600] * n_seq, nkv, hd, base=1e4, garbage=True)
+    start, cached = ints(*begin), ints(*[600] * n_seq)
+    before = c.pool.clone()
+    q, k = rows(1, T, nh, hd), rows(2, T, nkv, hd)
+    q_out = torch.full_like(q, 7.0)
+
+    def reported():
+        st = c.status()
+        assert st["code"] == _lib.FB_ERR_RANGE and st["where"] == 23 and begin[st["sequence"] + 1] < begin[st["sequence"]], st
+
+    c.append(0, k, k, cached, q=q, start=start, q_out=q_out)
+    reported()
+    assert (q_out == 7.0).all() and torch.equal(c.pool, before)
+    assert all((x == 0).all() for x in c.read(0, T, cached, start=start))
+    reported()
+    for hints in ({}, dict(max_new=1), dict(max_len=100000)):
+        c.attend(0, q, cached, start=start, out=q_out, **hints)
+        reported()
+        assert (q_out == 7.0).all()
