@@ -6,8 +6,9 @@
 // tiles take turns: one multiplies while the other exponentiates. Keys and values are dequantised once for both tiles by six warps into the K-major
 // 128-byte-swizzle layout that the MMA reads, K as [position][dim], V as [dim][position], each number (nib - 8) s + z rounded once. (Operands nib - 8, with s and z in the
 // softmax as kv4_attn_few has them, would be exact, but cost the softmax, which is what bounds this kernel, twice its instructions.) All operands are fp16, half a step
-// 2^-11: K times a power of two per step (per position where the keys of its 128 positions are more than 2^23 apart), Q times one per row, P times 2^7, V as it is. A page whose
-// rows of V have bounds 8 |s| + |z| outside [2^-10, 2^15) has its V and P in bf16, half a step 2^-8: there rows of any size stand side by side, whatever their weight.
+// 2^-11: K times a power of two per step (per position where the keys of its 128 positions are more than 2^23 apart), Q times one per row, P times 2^7, V as it is. A page with a
+// row of V whose values fp16 does not hold to 2^-11 of the largest one (below about 2^-13, and from 2^15 on) has its V and P in bf16, half a step 2^-8: there rows of any size stand
+// side by side, whatever their weight.
 // (With bf16 operands throughout 1000 tokens of 32 heads of 128 behind 7011 took 152 us, but outputs were off by 0.0044 of their 2-norm; now 166 us, 743 TFLOP/s, and 0.0017,
 // which is the rounding of the output itself. What is dearer is the factors' look and conversion, and P's second form. Tried and slower: factors converted in place by the
 // warp that brings the pages, 184 us, as it has no more than a step's time; P in either form behind a branch, 172 us.) Sums and maxima are fp32.
@@ -304,8 +305,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       uint8_t *kt = sm + M::K + b * M::KT, *vt = sm + M::V + 2 * b * M::VT;
       const int left0 = total - (task.unit + i) * kManyStep, left1 = left0 - kPage;                // positions of the pages that exist
       const bool none0 = s_none[r] != 0, none1 = s_none[r + 1] != 0 || left1 <= 0;
-      // Positions whose V is NaN: those, and what lies behind the last position, become zeros, as every row of P multiplies them. A page whose rows of V
-      // have bounds 8 |s| + |z| (its largest value that there can be) beyond [2^-10, 2^15) is `wide`; kmost, kleast: the largest bound of a key, the smallest but 0.
+      // Positions whose V is NaN: those, and what lies behind the last position, become zeros, as every row of P multiplies them. A page is `wide`
+      // whose rows of V have bounds 8 |s| + |z| (what a value may be at most, 17/15 of the largest one at most) beyond [2^-13, 2^15): half a step of fp16's smallest, 2^-25, is 2^-11
+      // of a row's largest value there. s has to be exact in fp16, as it is from 2^-17 on; below, what it is off by counts eight times, and the bound starts at 2^-10. kmost, kleast: the largest bound of a key, the smallest but 0.
       uint32_t kmost = 0, kleast = 0x7f800000u;
       bool wide0 = false, wide1 = false;
       auto look = [&](const uint8_t* rec, int left, bool& wide) {
@@ -321,7 +323,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
             if (kb > 0.f) kleast = min(kleast, __float_as_uint(kb));
           }
           bad[k] = __ballot_sync(0xffffffffu, in && !num);
-          wide |= __any_sync(0xffffffffu, in && num && vb != 0.f && !(vb >= 0x1p-10f && vb < 0x1p15f)) != 0;
+          const float vsa = fabsf(bflo(c)), low = vsa == 0.f || vsa >= 0x1p-17f ? 0x1p-13f : 0x1p-10f;
+          wide |= __any_sync(0xffffffffu, in && num && vb != 0.f && !(vb >= low && vb < 0x1p15f)) != 0;
         }
         return (unsigned long long)bad[0] | (unsigned long long)bad[1] << 32;
       };

@@ -35,27 +35,34 @@ def bounds(q, K, V, cached, scale, amask=None, many=False, wide=None):
     w = p ** 2 * score
     var = mix(w, v ** 2) - 2 * out * mix(w, v) + out ** 2 * w.sum(-1).T[..., None]
     if many:
+        # probability and value, each by half a step of its type. fp16's numbers below 2^-14 are 2^-24 apart: half a step of a value there is 2^-25 = 2^-11 2^-14
         h = torch.full((L,), FP16, dtype=torch.float64, device=q.device)
+        least = torch.full((L, 1, 1), 2.0 ** -14, dtype=torch.float64, device=q.device)
         if wide is not None:
-            h[wide] = BF16
-        var = var + mix(p ** 2 * (2 * h ** 2 / 3), v ** 2)
+            h[wide], least[wide] = BF16, 0.0
+        var = var + mix(p ** 2 * (h ** 2 / 3), v ** 2 + torch.maximum(v.abs(), least * (v != 0)) ** 2)
     else:
         span = v - v.amin(-1, keepdim=True)
         most = (p.unsqueeze(-1) * span.amax(-1).T[:, None, :, None]).amax(2)            # largest p s a row, [heads, n, 1]
         var = var + mix(p ** 2, span ** 2) * FP16 ** 2 / 3 + (L * (2.0 ** -25 * most) ** 2 / 3).transpose(0, 1)
     slack = 2.0 ** -18 * mix(p, v.abs())
+    if many:
+        # A row whose 16 numbers lie within 16 steps of the type: rows like it round alike, whatever their signs (z is not mirrored), so these errors are not independent
+        # and may add up to half a step of each: |sum p e| <= h sum p |v|.
+        alike = (v.amax(-1) - v.amin(-1)) <= 32 * h[:, None] * v.abs().amax(-1)
+        slack = slack + mix(p, v.abs() * (h[:, None] * alike)[..., None])
     out[spoiled] = math.nan
     return out, var.clamp(min=0).sqrt(), slack
 
 
 def check(got, want, sigma, slack):
     """Every element: half a step of bf16 and six times the root of mean squares. All of them together: what the mean squares add up to (a rounding's is a third
-    of half a step's square at most), a quarter more for few elements that hang together."""
+    of half a step's square at most), a quarter more for few elements that hang together, and on top of it what does not average out (norms of a sum: at most the sum)."""
     assert torch.equal(got.isnan(), want.isnan())
     fine = ~want.isnan()
     err, o, s = (got.double() - want)[fine], want[fine], sigma[fine]
     worst = float((err.abs() / (o.abs() * BF16 + 6 * s + slack[fine]).clamp(min=1e-300)).max()) if err.numel() else 0.0
-    whole = float(err.norm() / ((o * BF16) ** 2 / 3 + s ** 2).sum().sqrt().clamp(min=1e-300)) if err.numel() else 0.0
+    whole = float((err.norm() - slack[fine].norm()).clamp(min=0) / ((o * BF16) ** 2 / 3 + s ** 2).sum().sqrt().clamp(min=1e-300)) if err.numel() else 0.0
     assert worst <= 1.0, worst
     assert whole <= 1.25, whole
     return worst, whole

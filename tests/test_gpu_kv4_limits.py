@@ -226,3 +226,44 @@ def test_starts_that_go_down_leave_out_the_whole_call(T, order):
         c.attend(0, q, cached, start=start, out=q_out, **hints)
         reported()
         assert (q_out == 7.0).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------- values next to the border of fp16's range
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("largest,flat,wide", [(2.0 ** -10, False, False), (2.0 ** -11.5, False, False), (2.0 ** -12.7, False, False), (2.0 ** -12.7, True, False), (2.0 ** -14, False, True),
+                                               (2.0 ** -20, False, True), (2.0 ** -30, True, True), (2.0 ** 13, False, False), (2.0 ** 15, False, True)])
+def test_a_row_of_small_values_takes_no_bits_from_its_page(hd, largest, flat, wide):
+    """One row of every page of V has this largest number: down to 2^-13 its page stays in fp16."""
+    nh, nkv, cached, new = 8, 2, 600, 40
+    n = cached + new
+    v = rows(101, n, nkv, hd).float()
+    at = torch.arange(7, n, 64, device=DEV)
+    v[at] *= largest / v[at].abs().amax(-1, keepdim=True)
+    if flat:
+        v[at] = largest
+    c = make([n], nkv, hd, base=None, garbage=True)
+    c.append(0, rows(102, n, nkv, hd, 1.3), v.bfloat16(), 0)
+    K, V = c.read(0, n, 0)
+    q = rows(103, new, nh, hd)
+    out = c.attend(0, q, cached)
+    c.check()
+    kv4_bounds.check(out, *kv4_bounds.bounds(q, K, V, cached, hd ** -0.5, many=True, wide=torch.full((n,), wide, device=DEV)))
+
+
+@pytest.mark.parametrize("power", [-9.5, -11.0, -12.5])
+def test_rows_of_small_values_alone(power):
+    """All rows that small, close together or far apart: nothing larger hides what they lose."""
+    hd, nh, nkv, cached, new = 64, 8, 2, 300, 40
+    n = cached + new
+    for spread in (1.0, 0.1, 0.004):
+        base = torch.randn(n, nkv, 1, generator=gen(111), device=DEV).sign()
+        v = (base + spread * (torch.rand(n, nkv, hd, generator=gen(112), device=DEV) * 2 - 1)) / (1 + spread) * 2.0 ** power
+        c = make([n], nkv, hd, base=None, garbage=True)
+        c.append(0, rows(113, n, nkv, hd, 1.3), v.bfloat16(), 0)
+        K, V = c.read(0, n, 0)
+        q = rows(114, new, nh, hd)
+        out = c.attend(0, q, cached)
+        c.check()
+        # steps of these rows that fp16 does not hold (below 2^-17): their page is in bf16
+        narrow = 2 * spread / (1 + spread) * 2.0 ** power / 15 < 2.0 ** -16.9 and power < -9.9
+        kv4_bounds.check(out, *kv4_bounds.bounds(q, K, V, cached, hd ** -0.5, many=True, wide=torch.full((n,), narrow, device=DEV)))
