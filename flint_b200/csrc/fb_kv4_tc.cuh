@@ -36,11 +36,12 @@ struct Kv4Many {
   static_assert(TOTAL <= 227 * 1024 && T_O + 2 * HD <= TCOLS && QT % 1024 == 0 && VT % 1024 == 0 && RAW % 16 == 0 && REC % 16 == 0, "plan");
 };
 
-__device__ __forceinline__ uint32_t kv4_dequant2(uint32_t w, __nv_bfloat162 s, __nv_bfloat162 z) {       // nibbles in bits 0..3 and 16..19
-  const uint32_t x = (w & 0x000F000Fu) | 0x43004300u;            // 128 + nib
-  const uint32_t k136 = 0x43084308u;
-  const __nv_bfloat162 r = __hfma2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&k136)), s, z);
-  return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ __nv_bfloat162 kv4_bf2(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
+// nibbles in bits 0..3 and 16..19. A row that reaches the largest number rounds past it: not to an infinity, which would be NaN where the probability is 0
+__device__ __forceinline__ uint32_t kv4_dequant2(uint32_t w, __nv_bfloat162 s, __nv_bfloat162 z) {
+  const __nv_bfloat162 r = __hfma2(__hsub2(kv4_bf2((w & 0x000F000Fu) | 0x43004300u), kv4_bf2(0x43084308u)), s, z),        // 128 + nib - 136
+                       c = __hmax2(__hmin2(r, kv4_bf2(0x7f7f7f7fu)), kv4_bf2(0xff7fff7fu));
+  return *reinterpret_cast<const uint32_t*>(&c);
 }
 // ... fp16, nibbles in bits 0..3 and 16..19, or 4..7 and 20..23 (nib - 8 is exact, one rounding follows)
 __device__ __forceinline__ __half2 kv4_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
@@ -52,7 +53,6 @@ __device__ __forceinline__ uint32_t kv4_half_hi(uint32_t w, __half2 s, __half2 z
   const __half2 r = __hfma2(__hfma2(kv4_h2((w & 0x00F000F0u) | 0x64006400u), kv4_h2(0x2C002C00u), kv4_h2(0xD480D480u)), s, z);
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ __nv_bfloat162 kv4_bf2(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;

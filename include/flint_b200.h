@@ -247,7 +247,8 @@ int fb_gemv_static(const void* d_q, const void* d_s, const void* d_z, int32_t ro
  *                   (multiples of 8, 16-byte aligned). d_freq: device uint64 [head_dim / 2], turns per position in units of 2^-64 (half-split pairs), or NULL: no
  *                   rotation. d_depth: rotation position of a token behind its sequence's cached ones (tree nodes), or NULL: its place. d_q may be NULL
  *   fb_kv4_attend : d_out = softmax(scale * q K^T) V over the cached positions and the sequence's own new tokens, which have been appended: causal, or new token j
- *                   where d_amask[m * mask_ld + j] != 0 (m: token of the call). A token that sees nothing gets zeros. Sums are fp32: values of 2^112 and more may overflow them. max_new and max_len: about the
+ *                   where d_amask[m * mask_ld + j] != 0 (m: token of the call). A token that sees nothing gets zeros. Sums are fp32: values of 2^112 and more may overflow them, and scores of queries or keys
+ *                   of 2^117 and more may be none (of tokens that see them: others come out as if they were not there). max_new and max_len: about the
  *                   most new tokens and positions of a sequence; they decide how the work is cut, not what comes out.
  *                   d_work: scratch of fb_kv4_attend_bytes(the same seqs, n_head, max_new, max_len) bytes (0 for one sequence of up to 1344 positions and 64 query rows a
  *                   kv head), 16-byte aligned, this call's alone

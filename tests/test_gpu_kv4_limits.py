@@ -267,3 +267,41 @@ def test_rows_of_small_values_alone(power):
         # steps of these rows that fp16 does not hold (below 2^-17): their page is in bf16
         narrow = 2 * spread / (1 + spread) * 2.0 ** power / 15 < 2.0 ** -16.9 and power < -9.9
         kv4_bounds.check(out, *kv4_bounds.bounds(q, K, V, cached, hd ** -0.5, many=True, wide=torch.full((n,), narrow, device=DEV)))
+
+
+@pytest.mark.parametrize("hd", [64, 80, 128])
+@pytest.mark.parametrize("new", [9, 100])
+@pytest.mark.parametrize("masked", [False, True])
+def test_values_that_a_token_does_not_see_leave_it_alone(hd, new, masked):
+    """New tokens whose keys and values are the type's largest and smallest numbers, alone, among usual ones, and among others that take a row's numbers past the largest: tokens
+    ahead of them, or whose masks leave them out."""
+    nh, nkv, cached = 8, 2, 100
+    top, at = torch.finfo(torch.bfloat16).max, new // 2
+    for which in range(5):
+        k, v = rows(121, cached + new, nkv, hd), rows(122, cached + new, nkv, hd)
+        for x in (k, v):
+            row = x[cached + at]
+            if which < 2:
+                row[:] = top if which else -top
+            elif which == 2:
+                row[:, ::5] = -top
+            elif which == 3:
+                row[:] = 1.08e36
+                row[:, 3] = top
+            else:
+                row[:] = 0.0
+                row[:, 1::2] = top
+        c = make([cached + new], nkv, hd, base=None, garbage=True)
+        c.append(0, k, v, 0)
+        K, V = c.read(0, cached + new, 0)
+        q = rows(123, new, nh, hd, 1.5)
+        amask = torch.ones(new, new, dtype=torch.uint8, device=DEV).tril() if masked else None
+        if masked:
+            amask[:, at] = 0
+        out = c.attend(0, q, cached, amask=amask)
+        c.check()
+        blind = slice(0, new if masked else at)
+        K[cached + at], V[cached + at] = 0, 0              # the bounds' matrices multiply what is not seen by zero
+        wide = torch.zeros(cached + new, dtype=torch.bool, device=DEV)
+        wide[(cached + at) // 64 * 64:(cached + at) // 64 * 64 + 64] = True
+        kv4_bounds.check(out[blind], *(x[blind] for x in kv4_bounds.bounds(q, K, V, cached, hd ** -0.5, amask, many=new * nh // nkv > 64, wide=wide)))
