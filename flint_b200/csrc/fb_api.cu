@@ -8,6 +8,7 @@
 
 #include "../../include/flint_b200.h"
 #include "fb_ctx.hpp"
+#include "fb_kv4_geometry.hpp"
 #include "fb_decode.cuh"
 
 using namespace fb;
@@ -469,9 +470,16 @@ int fb_bind_kv4(fb_ctx* c, const fb_kv4_seqs* s, int64_t layer_bytes, const uint
   if (!c->kv4_new) FB_CUDA(c, dmalloc(&c->kv4_new, (size_t)2 * kPromptRows * d.n_kv_head * d.head_dim * 2));
   if (!c->kv4_logits) FB_CUDA(c, dmalloc(&c->kv4_logits, (size_t)d.vocab * 4));
   if (!c->kv4_token) FB_CUDA(c, dmalloc(&c->kv4_token, 4));
-  if (!c->kv4_work) {
-    c->kv4_work_bytes = kv4_attend_most(d.n_kv_head, d.head_dim, c->sm_count);
-    FB_CUDA(c, dmalloc(&c->kv4_work, c->kv4_work_bytes));
+  const size_t need = attend_most(d.n_kv_head, d.n_head / d.n_kv_head, d.head_dim, (int64_t)s->table_ld * 64, kPromptRows, c->sm_count);
+  if (need > c->kv4_work_bytes) {                              // twice what there was, at least: the places for smaller ones do not run out
+    float* work;
+    const size_t bytes = need > 2 * c->kv4_work_bytes ? need : 2 * c->kv4_work_bytes;
+    constexpr int places = sizeof(c->kv4_work) / sizeof(c->kv4_work[0]);
+    if (c->kv4_work[places - 1]) return FB_ERR_STATE;
+    FB_CUDA(c, dmalloc(&work, bytes));
+    for (int i = places - 1; i > 0; i--) c->kv4_work[i] = c->kv4_work[i - 1];
+    c->kv4_work[0] = work;
+    c->kv4_work_bytes = bytes;
   }
   c->kv4 = *s;
   c->kv4.d_start = c->kv4.d_cached = nullptr;

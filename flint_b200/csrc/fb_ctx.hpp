@@ -45,8 +45,8 @@ struct fb_ctx {
   uint16_t* kv4_new;                                                // ... a layer's new keys and values ahead of their rounding, bf16 [2][kPromptRows][n_kv * HD],
   float* kv4_logits;                                                // and what a decode step on it needs: logits, token
   int32_t* kv4_token;
-  float* kv4_work;                                                  // scratch of its attention
-  size_t kv4_work_bytes;
+  float* kv4_work[16];                                              // scratch of its attention: the one in use, and smaller ones of caches bound before, which
+  size_t kv4_work_bytes;                                            // captured passes may still name
 };
 
 inline bool has_kv(const fb_ctx* c) { return c->kv4_bound || c->kc; }
@@ -97,10 +97,9 @@ cudaError_t pass_bind_matrix(fb_ctx* c, int which, const void* q, const void* s,
 // one decode step on the 4-bit cache: the M-token pass with one token, and the arg-max
 int pass_decode(fb_ctx* c, int32_t token, const int32_t* d_token, void* d_h, int32_t pos, float* d_logits, int32_t* d_next, cudaStream_t st);
 
-// ---- the 4-bit cache (fb_kv4.cu), with the context's limit of waits, and the most scratch that it asks for with one sequence
-size_t kv4_attend_most(int n_kv_head, int head_dim, int sms);
+// ---- the 4-bit cache (fb_kv4.cu), with the context's limit of waits. fit: with less scratch than it would like the positions are not shared (else FB_ERR_ARG)
 int kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n_head, int32_t max_new, int32_t max_len, const uint8_t* d_amask, int32_t mask_ld,
-               float scale, void* d_out, int64_t o_ld, float* work, size_t work_bytes, unsigned spin_limit, cudaStream_t st);
+               float scale, void* d_out, int64_t o_ld, float* work, size_t work_bytes, bool fit, unsigned spin_limit, cudaStream_t st);
 
 // ---- the decode kernels of tensor-parallel ranks (fb_decode_tp.cu), by index into fb_api.cu's table
 const void* decode_tp_kernel(int id);

@@ -5,14 +5,12 @@
 #include "../../include/flint_b200.h"
 #include "fb_ctx.hpp"
 #include "fb_kv4.cuh"
+#include "fb_kv4_geometry.hpp"
 #include "fb_kv4_tc.cuh"
 
 using namespace fb;
 
 namespace {
-
-constexpr int kFewRows = 64;
-constexpr int kFewWarps = 7;                       // that compute, of a CTA of kv4_attn_few; an SM holds two CTAs
 
 int device_sms(int dev) {
   static int sms[64] = {};
@@ -46,51 +44,6 @@ int take_seqs(const fb_kv4_seqs* s, int rows_of_tokens, Kv4Seqs& S) {
   return FB_OK;
 }
 int done(cudaError_t e) { return e == cudaSuccess ? FB_OK : FB_ERR_CUDA; }
-
-// How an attention is cut. rows: query rows of a group; groups: of all sequences, at most; ctas: of a grid without clusters, at most.
-// Up to kFewRows query rows a kv head: kv4_attn_few in groups of 8 or 16 rows, which dequantise the cache anew for each group. More: kv4_attn_many. Microseconds, few /
-// many: 16 tokens of 4 heads (64 rows) behind 1024 positions 9.9 / 13.5, behind 4000 14.5 / 17.5, 12 (48 rows) behind 8000 24.2 / 23.9; 26 tokens (104 rows) behind
-// 1024 13.5 / 13.2, behind 8000 44 / 26; 61 (244 rows) behind 3001 46 / 28.
-// Few: a group's positions are shared by a cluster (one launch) while a warp of a cluster of eight has no more than six units; by as many CTAs as the GPU holds and a
-// second launch that joins them, beyond that. (With one CTA of 16-row groups per SM the GPU holds 15 clusters of 8, but 36 of 4.) One sequence, eight
-// kv heads, cluster / second launch: 1000 positions 5.5 / 8.2, 4000 6.7 / 8.5, 32768 20.5 / 13.1 (heads of 80). Of a batch no positions are shared until a
-// warp would have more than 12 units: 48 sequences of up to 2000 positions 17.8 / 22.7, 24 of up to 8000 51 / 18.3 (over 148 parts; over 296 22.1).
-// Many: a task has 128 or 256 query rows. A step of 128 positions takes about 2.5 us (1.6 with one tile of 128 rows), a task about two steps more, the second launch 5 us and what the
-// partials take to write and read; rows and parts of the smallest sum are taken. 1000 tokens of 4 heads behind 7011 positions, 160 items of 256 rows on 148 SMs: whole
-// 253, four parts 216; 128 items: whole 160, two parts 197. 61-node tree of 4 heads behind 3001: eight items of 256 rows whole 71, eight parts 28.3, 24 parts 42; sixteen of
-// 128 rows in eight parts 23.8. A prompt of 200 tokens: 12.4 with 256 rows, 10.5 with 128.
-struct Kv4Geometry { int rows; int64_t groups, ctas; int nsplit, slots, chunk; };
-Kv4Geometry few_geometry(int n_seq, int n_tokens, int nkv, int r, int max_new, int max_len, int sms) {
-  Kv4Geometry g{(int64_t)max_new * r <= 8 ? 8 : 16, 0, 0, 1, 0, 8};
-  auto groups_of = [&](int rows) { return n_seq == 1 ? ((int64_t)n_tokens * r + rows - 1) / rows : (int64_t)n_tokens * r / rows + n_seq; };
-  const bool many = (int64_t)max_new * r > kFewRows;
-  const int64_t units = ((int64_t)max_len + 31) / 32, steps = ((int64_t)max_len + kManyStep - 1) / kManyStep;
-  if (many) {
-    g.chunk = 1;
-    double best = 0;
-    for (int rows : {kManyRows / 2, kManyRows}) {
-      const double step_us = rows == kManyRows && (int64_t)max_new * r > kManyRows / 2 ? 2.5 : 1.6;
-      const int64_t items = groups_of(rows) * nkv;
-      for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24}) {
-        if (parts > steps || (parts > 1 && items * parts > 3 * sms)) break;
-        const int64_t per = (steps + parts - 1) / parts, tasks = items * ((steps + per - 1) / per);
-        const double us = (double)((tasks + sms - 1) / sms) * (double)(per + 2) * step_us + (parts > 1 ? 5.0 + (double)tasks * rows * 1056 / 3e6 : 0.0);
-        if (best == 0 || us < best) { best = us; g.rows = rows; g.slots = parts > 1 ? (int)(items * parts) : 0; }
-      }
-    }
-  }
-  g.groups = groups_of(g.rows);
-  const int64_t items = g.groups * nkv;
-  if (!many && n_seq == 1) {
-    while (g.nsplit < 8 && items * g.nsplit * 2 <= (g.nsplit == 4 ? sms * 2 / 3 : sms) && units >= g.nsplit * 2 * 4) g.nsplit *= 2;
-    if (units > (int64_t)6 * kFewWarps * g.nsplit && items * g.nsplit <= sms) { g.nsplit = 1; g.slots = 2 * sms; }
-  } else if (!many && units > 12 * kFewWarps && items <= 8 * (int64_t)sms) {
-    g.slots = sms;
-  }
-  g.ctas = items + g.slots;
-  return g;
-}
-size_t few_work(const Kv4Geometry& g, int hd) { return g.slots ? (size_t)g.ctas * g.rows * (hd + 4) * 4 : 0; }
 
 // rows of 16-bit numbers that are read 16 bytes at a time
 bool rows_ok(const void* p, int64_t ld, int64_t width) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld >= width; }
@@ -247,13 +200,13 @@ int fb_kv4_move(const fb_kv4_seqs* s, int32_t n_layer, int64_t layer_bytes, cons
 
 int fb_kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n_head, int32_t max_new, int32_t max_len, const uint8_t* d_amask,
                   int32_t mask_ld, float scale, void* d_out, int64_t o_ld, void* d_work, size_t work_bytes, void* stream) {
-  return kv4_attend(s, d_q, q_ld, n_head, max_new, max_len, d_amask, mask_ld, scale, d_out, o_ld, (float*)d_work, work_bytes, 4000000u, (cudaStream_t)stream);
+  return kv4_attend(s, d_q, q_ld, n_head, max_new, max_len, d_amask, mask_ld, scale, d_out, o_ld, (float*)d_work, work_bytes, false, 4000000u, (cudaStream_t)stream);
 }
 
 }  // extern "C"
 
 int kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n_head, int32_t max_new, int32_t max_len, const uint8_t* d_amask, int32_t mask_ld,
-               float scale, void* d_out, int64_t o_ld, float* work, size_t work_bytes, unsigned spin_limit, cudaStream_t st) {
+               float scale, void* d_out, int64_t o_ld, float* work, size_t work_bytes, bool fit, unsigned spin_limit, cudaStream_t st) {
   Kv4Attend p;
   const int rc = take_seqs(s, 1, p.S);
   if (rc != FB_OK) return rc;
@@ -268,8 +221,9 @@ int kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n_he
   p.q = (const uint16_t*)d_q; p.out = (uint16_t*)d_out; p.q_ld = q_ld; p.o_ld = o_ld; p.amask = d_amask; p.mask_ld = mask_ld;
   p.nh = n_head; p.R = n_head / s->n_kv_head;
   p.scale = scale * 1.4426950408889634f; p.spin_limit = spin_limit;
-  const Kv4Geometry geo = few_geometry(s->n_seq, s->n_tokens, s->n_kv_head, p.R, max_new < s->n_tokens ? max_new : s->n_tokens, max_len, sms);
-  if (few_work(geo, s->head_dim) > work_bytes || ((uintptr_t)work & 15)) return FB_ERR_ARG;
+  Kv4Geometry geo = attend_geometry(s->n_seq, s->n_tokens, s->n_kv_head, p.R, max_new < s->n_tokens ? max_new : s->n_tokens, max_len, sms);
+  if (fit && attend_work(geo, s->head_dim) > work_bytes) geo = whole(geo, s->n_kv_head);
+  if (attend_work(geo, s->head_dim) > work_bytes || ((uintptr_t)work & 15)) return FB_ERR_ARG;
   p.work = work;
   switch (s->head_dim) {
     case 64: return done(launch_attend<64>(p, geo, st));
@@ -278,12 +232,9 @@ int kv4_attend(const fb_kv4_seqs* s, const void* d_q, int64_t q_ld, int32_t n_he
   }
 }
 
-// one sequence: few rows are split while their groups are fewer than the SMs, into two parts an SM more; many rows into three an SM at most
-size_t kv4_attend_most(int n_kv_head, int head_dim, int sms) { return (size_t)(5 * sms) * kManyRows * (head_dim + 4) * 4; }
-
 size_t fb_kv4_attend_bytes(const fb_kv4_seqs* s, int32_t n_head, int32_t max_new, int32_t max_len) {
   if (!s || s->n_kv_head < 1 || s->n_kv_head > 65535 || n_head < 1 || n_head % s->n_kv_head || max_new < 1 || max_len < 1 || s->n_seq < 0) return 0;
   const int sms = device_sms(s->device);
   if (!sms) return 0;
-  return few_work(few_geometry(s->n_seq, s->n_tokens, s->n_kv_head, n_head / s->n_kv_head, max_new < s->n_tokens ? max_new : s->n_tokens, max_len, sms), s->head_dim);
+  return attend_work(attend_geometry(s->n_seq, s->n_tokens, s->n_kv_head, n_head / s->n_kv_head, max_new < s->n_tokens ? max_new : s->n_tokens, max_len, sms), s->head_dim);
 }

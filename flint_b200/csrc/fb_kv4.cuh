@@ -16,6 +16,7 @@
 
 #include "fb_common.cuh"
 #include "fb_drain.hpp"
+#include "fb_kv4_geometry.hpp"
 
 namespace fb {
 
@@ -541,7 +542,7 @@ __device__ __forceinline__ void kv4_finish(const Kv4Attend& P, const Kv4Seq& seq
 // than a cluster leave them to kv4_join.
 template <int HD, int NQ, int W>
 struct Kv4Few {
-  static constexpr int U = 32, NST = 3, ROWS = 8 * NQ, PW = HD + 4;         // positions of a unit, stages of a warp, query rows, floats of a partial
+  static constexpr int U = kFewUnit, NST = 3, ROWS = 8 * NQ, PW = HD + 4;         // positions of a unit, stages of a warp, query rows, floats of a partial
   static constexpr int STAGE = U / 16 * Kv4<HD>::BLOCK, RING = W * NST * STAGE, PART = W * ROWS * PW * 4;
   static constexpr int INBOX = RING > PART ? RING : PART;
   static constexpr int BAR = INBOX + 16 * PW * 4, SKIP = BAR + 2 * W * NST * 8, TOTAL = SKIP + W * NST * 4 + 16;

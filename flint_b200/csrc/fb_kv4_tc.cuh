@@ -16,11 +16,12 @@
 // Warps: 0..3 and 4..7 softmax of tiles 0 and 1 (and Q in, O out), 8..13 dequantise, 14 brings pages (one bulk copy each), 15 issues MMAs.
 #pragma once
 #include "fb_kv4.cuh"
+#include "fb_kv4_geometry.hpp"
 #include "fb_tcgen.cuh"
 
 namespace fb {
 
-constexpr int kManyThreads = 16 * 32, kManyRows = 256, kManyStep = 128;
+constexpr int kManyThreads = 16 * 32;
 constexpr float kManyLift = 7.f;                   // probabilities are 2^7 times what they are, 2^15 at most: in fp16 they lose nothing down to 2^-21
 constexpr int kManyDequant = 6;                    // warps that dequantise
 

@@ -155,7 +155,7 @@ int run_tc_pass(fb_ctx* c, const int32_t* d_tokens, const void* d_h, const int32
     if (kv4) {
       int rc = fb_kv4_append(&seqs, c->vq, QD, kcl, kw, vcl, kw, d.n_head, d_depth, c->kv4_freq, c->vq, QD, st);
       if (rc == FB_OK)
-        rc = kv4_attend(&seqs, c->vq, QD, d.n_head, M, pos + M, d_amask, M, d.attn_scale, c->vao, QD, c->kv4_work, c->kv4_work_bytes, c->spin_limit, st);
+        rc = kv4_attend(&seqs, c->vq, QD, d.n_head, M, pos + M, d_amask, M, d.attn_scale, c->vao, QD, c->kv4_work[0], c->kv4_work_bytes, true, c->spin_limit, st);
       if (rc != FB_OK) return rc == FB_ERR_CUDA ? cuda_fail(c, cudaGetLastError()) : rc;
       seqs.d_pool = (uint8_t*)seqs.d_pool + c->kv4_layer;
     } else {
@@ -225,8 +225,10 @@ cudaError_t pass_alloc(fb_ctx* c) {
 
 void pass_free(fb_ctx* c) {
   void* ptrs[] = {c->vh, c->vxn, c->vq, c->vao, c->vact, c->t_qkv, c->t_o, c->t_gu, c->t_d, c->t_lm, c->vrope,
-                  c->vfx, c->vfao, c->vfa, c->vfa_inv, c->vamax, c->gu_norms, c->kv4_new, c->kv4_logits, c->kv4_token, c->kv4_work};
+                  c->vfx, c->vfao, c->vfa, c->vfa_inv, c->vamax, c->gu_norms, c->kv4_new, c->kv4_logits, c->kv4_token};
   for (void* p : ptrs)
+    if (p) cudaFree(p);
+  for (float* p : c->kv4_work)
     if (p) cudaFree(p);
 }
 

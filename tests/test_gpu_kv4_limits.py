@@ -7,6 +7,7 @@ import torch
 from flint_b200 import _lib, packing
 from flint_b200.config import ModelArgs
 from flint_b200.engine import DecodeEngine
+from flint_b200.kv4 import KvCache4
 from tests import kv4_bounds
 from tests.test_gpu_kv4 import check_attention, filled, gen, ints, make, rows
 
@@ -305,3 +306,44 @@ def test_values_that_a_token_does_not_see_leave_it_alone(hd, new, masked):
         wide = torch.zeros(cached + new, dtype=torch.bool, device=DEV)
         wide[(cached + at) // 64 * 64:(cached + at) // 64 * 64 + 64] = True
         kv4_bounds.check(out[blind], *(x[blind] for x in kv4_bounds.bounds(q, K, V, cached, hd ** -0.5, amask, many=new * nh // nkv > 64, wide=wide)))
+
+
+def test_scratch_of_an_engine_goes_by_its_cache():
+    """A short cache takes next to none; a longer one bound later has what its passes need, and a pass captured over the short one still has its own."""
+    cfg = ModelArgs.from_name("tiny")
+    packed = packing.synth_packed(cfg, 0, device=DEV)
+    nkv, hd = cfg.n_local_heads, cfg.head_dim
+
+    def cache(slots):
+        c = KvCache4(cfg.n_layer, slots // 64, nkv, hd, torch.arange(slots // 64, dtype=torch.int32, device=DEV)[None], rope_base=cfg.rope_base)
+        for layer in range(cfg.n_layer):
+            c.append(layer, rows(layer, slots - 640, nkv, hd), rows(layer + 9, slots - 640, nkv, hd), 0)
+        return c
+    short, middle, long = cache(704), cache(8000), cache(32000)
+    eng = DecodeEngine(cfg, packed, max_seq=64)
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    eng.bind_kv4(short)
+    assert free - torch.cuda.mem_get_info()[0] < 12e6
+    tok, out = torch.tensor([7], dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    eng.decode_chained(tok, 64, out)
+    want = out.clone()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        eng.decode_chained(tok, 64, out)
+    toks = torch.arange(5, 605, dtype=torch.int32, device=DEV)
+    for c in (middle, long, middle):
+        eng.bind_kv4(c)
+        for n in (1, 40, 300, 600):
+            pos = c.slots - 640
+            got = eng.decode(5, pos) if n == 1 else eng.prefill(toks[:n], pos)[0]
+            fresh = DecodeEngine(cfg, packed, kv_bits=4, cache=c)
+            again = fresh.decode(5, pos) if n == 1 else fresh.prefill(toks[:n], pos)[0]
+            fresh.check()
+            assert torch.equal(got, again)
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    eng.check()
+    assert torch.equal(out, want)
