@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
           tc_mma_ss(tmem + M::T_S + t * 128, q0 + (uint64_t)(t * (M::QT >> 4)) + off, kb + off, id, k ? 1u : 0u);
         }
         tc_commit(&s_full[t]);
-        if (t == tiles - 1) tc_commit(&k_empty[i & 1]);
+        if (t == tiles - 1 && i + 2 < n) tc_commit(&k_empty[i & 1]);       // step i + 2 waits for it: none is issued that nobody waits for before the CTA ends
       }
       __syncwarp();
     };
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
         }
         if (h) {
           tc_commit(&pv_done[t]);
-          if (t == tiles - 1) tc_commit(&v_empty[i & 1]);
+          if (t == tiles - 1 && i + 2 < n) tc_commit(&v_empty[i & 1]);
         }
       }
       __syncwarp();

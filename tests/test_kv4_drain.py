@@ -3,6 +3,7 @@ as late as it can: nothing may be in flight behind it, and no wait may be one th
 import ctypes
 import itertools
 import os
+import re
 import subprocess
 
 import pytest
@@ -92,3 +93,14 @@ def test_the_model_shows_the_orders_that_do_not_do():
     b.armed, b.over = 4, 4
     b.wait(0)
     assert b.hung
+
+
+def test_no_arrival_is_left_that_nobody_waits_for():
+    """The places of K and V are waited for from the third step on, two steps behind the products that free them: products of the last two steps announce nothing, or the
+    announcement could come after the CTA has ended."""
+    with open(os.path.join(CSRC, "fb_kv4_tc.cuh")) as f:
+        code = re.sub(r"//[^\n]*", "", f.read())
+    for bar in ("k_empty", "v_empty"):
+        assert re.findall(r"if \(([^;{}]*)\)\s*tc_commit\(&%s\b" % bar, code) == ["t == tiles - 1 && i + 2 < n"] and code.count("tc_commit(&" + bar) == 1
+        assert re.findall(r"if \(([^;{}]*)\) ok = __all_sync\(0xffffffffu, mbar_wait\(&%s\[b\], before" % bar, code) == ["i >= 2"]
+    assert "before = (uint32_t)((i >> 1) - 1) & 1u" in code
