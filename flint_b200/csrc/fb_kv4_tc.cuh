@@ -332,6 +332,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       // The usual case at a glance: whole pages, all factors within narrower bounds than that: s of V from 2^-13 to below 2^11, |z| below 2^14, of K s from 2^-12 on and
       // the same above.
       unsigned long long bad0 = 0, bad1 = 0;
+      bool looked = false;
       {
         const uint8_t* at = rec0 + (lane >> 4) * C::BLOCK + (lane & 15) * 4;
         uint32_t km = 0, vm = 0, ks = 0xffffu, vs = 0xffffu;
@@ -348,6 +349,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
         if (__all_sync(0xffffffffu, usual) && !none0 && !none1 && left1 >= kPage) {
           kmost = __float_as_uint(fmaf(8.f, bflo(km), bfhi(km)));
         } else {
+          looked = true;
           if (!none0) bad0 = look(rec0, left0, wide0);
           if (!none1) bad1 = look(rec1, left1, wide1);
         }
@@ -355,7 +357,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv4_attn_many(const Kv4Attend
       // One power of two does for keys whose bounds are 2^24 apart or less (fp16 then holds them from 2^-10 on); beyond that each has its own, so that a key
       // that is not seen, or as nothing to the softmax, takes no bits from the others.
       const uint32_t kmax = __reduce_max_sync(0xffffffffu, kmost);
-      const bool apart = __any_sync(0xffffffffu, (kmax >> 23) > (kleast >> 23) + 23u);
+      const bool apart = looked && __any_sync(0xffffffffu, (kmax >> 23) > (kleast >> 23) + 23u);
       const float2 kp = pow2_for(__uint_as_float(kmax));         // the largest into [2^14, 2^15)
       kf = kp.x;
       const bool special = none0 || none1 || bad0 || bad1 || left1 < kPage || wide0 || wide1;
