@@ -21,9 +21,10 @@ constexpr int kManyRows = 256, kManyStep = 128;    // of kv4_attn_many: most que
 // kv heads, cluster / second launch: 1000 positions 5.5 / 8.2, 4000 6.7 / 8.5, 32768 20.5 / 13.1 (heads of 80). Of a batch no positions are shared until a
 // warp would have more than 12 units: 48 sequences of up to 2000 positions 17.8 / 22.7, 24 of up to 8000 51 / 18.3 (over 148 parts; over 296 22.1).
 // Many: a task has 128 or 256 query rows. A step of 128 positions takes about 2.5 us (1.6 with one tile of 128 rows), a task about two steps more, the second launch 5 us and what the
-// partials take to write and read; rows and parts of the smallest sum are taken. 1000 tokens of 4 heads behind 7011 positions, 160 items of 256 rows on 148 SMs: whole
-// 253, four parts 216; 128 items: whole 160, two parts 197. 61-node tree of 4 heads behind 3001: eight items of 256 rows whole 71, eight parts 28.3, 24 parts 42; sixteen of
-// 128 rows in eight parts 23.8. A prompt of 200 tokens: 12.4 with 256 rows, 10.5 with 128.
+// partials take to write and read; rows and parts of the smallest sum are taken (all rows are counted with all positions, of which a prompt's first ones see fewer). 1000 tokens of
+// 4 heads behind 7011 positions on 148 SMs: eight kv heads, 128 items of 256 rows, whole 168, two parts 206, with 128 rows 262; ten kv heads, 160 items, whole 307, three parts
+// 277. Tree of 61 of 4 heads behind 3001, eight kv heads: 128 rows whole 58, eight parts 21.8, twelve 32; 256 rows in twelve parts 25.6. Tree of 26 behind 1024: whole 22.8,
+// six parts 13.3. A prompt of 200 tokens: 11.1 with 128 rows, 13.1 with 256.
 // rows of a group, groups, CTAs of a grid without clusters; CTAs of a cluster; tasks that all positions are cut into (0: they are not), of `chunk` units or more
 struct Kv4Geometry { int rows; int64_t groups, ctas; int nsplit, slots, chunk; };
 inline Kv4Geometry attend_geometry(int n_seq, int n_tokens, int nkv, int r, int max_new, int max_len, int sms) {

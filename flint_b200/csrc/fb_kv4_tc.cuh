@@ -1,18 +1,18 @@
 // Attention of many query rows over the paged 4-bit cache on the 5th-generation tensor cores (tcgen05): prompts and large trees.
 //
-// A CTA takes 256 query rows (row = token * R + head of the group) of a sequence and kv head as two tiles of 128 (or 128 rows, where the SMs are not filled otherwise), and its task's positions in steps of
-// 128 (two pages). Per step and tile: S[128 rows][128 positions] = Q K^T into tensor memory, softmax by a warpgroup (a thread a row: no shuffles), P back
+// A CTA takes 256 query rows (row = token * R + head of the group) of a sequence and kv head as two tiles of 128 (or 128 rows, where the SMs are not filled otherwise), and its
+// task's positions in steps of 128 (two pages). Per step and tile: S[128 rows][128 positions] = Q K^T into tensor memory, softmax by a warpgroup (a thread a row: no shuffles), P back
 // into tensor memory over S, O[128][HD] += P V. Tensor pipe and exponentials (16 a clock and SM) need the same 1024 clocks a tile and step at heads of 128, so the two
 // tiles take turns: one multiplies while the other exponentiates. Keys and values are dequantised once for both tiles by six warps into the K-major
 // 128-byte-swizzle layout that the MMA reads, K as [position][dim], V as [dim][position], each number (nib - 8) s + z rounded once. (Operands nib - 8, with s and z in the
-// softmax as kv4_attn_few has them, would be exact, but cost the softmax, which is what bounds this kernel, twice its instructions.) All operands are fp16, half a step
-// 2^-11: K times a power of two per step (per position where the keys of its 128 positions are more than 2^23 apart), Q times one per row, P times 2^7, V as it is. A page with a
-// row of V whose values fp16 does not hold to 2^-11 of the largest one (below about 2^-13, and from 2^15 on) has its V and P in bf16, half a step 2^-8: there rows of any size stand
-// side by side, whatever their weight.
-// (With bf16 operands throughout 1000 tokens of 32 heads of 128 behind 7011 took 152 us, but outputs were off by 0.0044 of their 2-norm; now 166 us, 743 TFLOP/s, and 0.0017,
-// which is the rounding of the output itself. What is dearer is the factors' look and conversion, and P's second form. Tried and slower: factors converted in place by the
-// warp that brings the pages, 184 us, as it has no more than a step's time; P in either form behind a branch, 172 us.) Sums and maxima are fp32.
-// The maximum is moved, and O rescaled, only when a score exceeds it by more than 2^8.
+// softmax as kv4_attn_few has them, would be exact, but cost the softmax, which is what bounds this kernel, twice its instructions.)
+// Operands are fp16, half a step 2^-11: K times a power of two per step (per position where the keys of its 128 positions are more than 2^23 apart), Q times one per row, P times 2^7,
+// V as it is. A page with a row of V whose values fp16 does not hold to 2^-11 of the largest one (below about 2^-13, and from 2^15 on) has its V and P in bf16, half a step 2^-8: there
+// rows of any size stand side by side, whatever their weight. Outputs are off by 0.0017 of their 2-norm, which is the rounding of the output itself. (bf16 throughout takes 9 % less
+// time: no look at the factors, no second form of P; but outputs are off by 0.0044. The factors converted in place by the warp that brings the pages: 10 % more, it has no
+// more than a step's time.) Sums and maxima are fp32. The maximum is moved, and O rescaled, only when a score exceeds it by more than 2^8.
+// 1000 tokens of 32 heads of 128 behind 7011 positions: 168 us, 735 TFLOP/s. No unit is full (tensor pipe 42 % of the time on a busy SM, exponentials 54 %): a tile's chain scores, maximum,
+// exponentials, P, PV is longer than what the other tile hides. Times move by up to 5 % with where the compiler places code that never runs.
 // Warps: 0..3 and 4..7 softmax of tiles 0 and 1 (and Q in, O out), 8..13 dequantise, 14 brings pages (one bulk copy each), 15 issues MMAs.
 #pragma once
 #include "fb_kv4.cuh"

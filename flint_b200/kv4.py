@@ -170,7 +170,8 @@ class KvCache4:
         """softmax(scale * q K^T) V of the new tokens q bf16 [T, heads, head_dim], whose keys and values have been appended, over the cached positions and the new
         tokens of their own sequence: causal, or those with amask[m, j] != 0 (uint8 or bool [T, new tokens of a sequence], j counted from the sequence's first
         new token). max_new: no sequence has more new tokens (default: T); max_len: about the longest sequence, for cutting the work (default: what `cached`
-        says, or all slots). A token that sees nothing gets zeros."""
+        says, or all slots). A token that sees nothing gets zeros. Probabilities (times a row's s) are rounded to fp16, beyond 64 query rows a kv head keys and values too
+        (bf16 in pages with very small or large values); scores and sums are fp32: include/flint_b200.h."""
         q, q_at, T, q_ld = self._rows(q, None, "q")
         heads = q.shape[1]
         if heads == 0 or heads % self.n_kv:

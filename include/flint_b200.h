@@ -247,12 +247,14 @@ int fb_gemv_static(const void* d_q, const void* d_s, const void* d_z, int32_t ro
  *                   (multiples of 8, 16-byte aligned). d_freq: device uint64 [head_dim / 2], turns per position in units of 2^-64 (half-split pairs), or NULL: no
  *                   rotation. d_depth: rotation position of a token behind its sequence's cached ones (tree nodes), or NULL: its place. d_q may be NULL
  *   fb_kv4_attend : d_out = softmax(scale * q K^T) V over the cached positions and the sequence's own new tokens, which have been appended: causal, or new token j
- *                   where d_amask[m * mask_ld + j] != 0 (m: token of the call). A token that sees nothing gets zeros. Sums are fp32: values of 2^112 and more may overflow them, and scores of queries or keys
- *                   of 2^117 and more may be none (of tokens that see them: others come out as if they were not there). max_new and max_len: about the
- *                   most new tokens and positions of a sequence; they decide how the work is cut, not what comes out.
+ *                   where d_amask[m * mask_ld + j] != 0 (m: token of the call). A token that sees nothing gets zeros. max_new and max_len: about the most new tokens and positions of a
+ *                   sequence; they decide how the work is cut, and so which of these roundings there are, beside the output's to bf16. Scores, maxima and sums are
+ *                   fp32 throughout. Up to 64 query rows a kv head (max_new * n_head / n_kv_head): keys and values as they are, probability times s in fp16. More: keys,
+ *                   values and probabilities in fp16, values and probabilities of a page in bf16 where one of its rows of values is smaller than about 2^-13 (and not
+ *                   zero) or 2^15 and larger. Values of 2^112 and more may overflow the sums, and scores of queries or keys of 2^117 and more may be NaN, for
+ *                   tokens that see them: others come out as if they were not there. Equal calls give equal bits.
  *                   d_work: scratch of fb_kv4_attend_bytes(the same seqs, n_head, max_new, max_len) bytes (0 for one sequence of up to 1344 positions and 64 query rows a
- *                   kv head), 16-byte aligned, this call's alone
- *                   until it has run
+ *                   kv head), 16-byte aligned, this call's alone until it has run
  *   fb_kv4_read   : f32 [n_layer][n_tokens][n_kv_head][head_dim], the numbers that the new tokens' rows stand for, bit for bit (tokens that
  *                   no sequence has, or whose page is none: zeros). d_k or d_v may be NULL
  *   fb_kv4_compact: fb_kv_compact on sequence 0: slot cached + i takes slot cached + path[i], i = 1 .. len-1, in order; most: entries of the path in d_accept
