@@ -41,6 +41,8 @@ def bounds(q, K, V, cached, scale, amask=None, many=False, wide=None):
         if wide is not None:
             h[wide], least[wide] = BF16, 0.0
         var = var + mix(p ** 2 * (h ** 2 / 3), v ** 2 + torch.maximum(v.abs(), least * (v != 0)) ** 2)
+        # ... and a probability is 2^7 times what it is there: half a step below 2^-14 is 2^-32 of the largest one
+        var = var + mix(see.double().expand_as(p) * (2.0 ** -64 / 3), v ** 2)
     else:
         span = v - v.amin(-1, keepdim=True)
         most = (p.unsqueeze(-1) * span.amax(-1).T[:, None, :, None]).amax(2)            # largest p s a row, [heads, n, 1]
