@@ -168,7 +168,7 @@ int fb_kv4_compact(const fb_kv4_seqs* s, int32_t n_layer, int64_t layer_bytes, c
   memset(&p, 0, sizeof(p));
   const int rc = take_seqs(s, 0, p.S);
   if (rc != FB_OK) return rc;
-  if (!d_accept || ((uintptr_t)d_accept & 3) || most < 0 || n_layer < 1 || n_layer > 65535 || layer_bytes < 0 || layer_bytes % 16 || s->d_cached) return FB_ERR_ARG;
+  if (s->n_seq < 1 || !d_accept || ((uintptr_t)d_accept & 3) || most < 0 || n_layer < 1 || n_layer > 65535 || layer_bytes < 0 || layer_bytes % 16 || s->d_cached) return FB_ERR_ARG;
   if (s->cached > s->table_ld * kPage - 1) return FB_ERR_RANGE;
   OnDevice g(s->device);
   if (!g.ok) return FB_ERR_CUDA;
@@ -181,7 +181,7 @@ int fb_kv4_move(const fb_kv4_seqs* s, int32_t n_layer, int64_t layer_bytes, cons
   memset(&p, 0, sizeof(p));
   const int rc = take_seqs(s, 0, p.S);
   if (rc != FB_OK) return rc;
-  if (n < 0 || (n > 0 && (!src || !dst)) || n_layer < 1 || n_layer > 65535 || layer_bytes < 0 || layer_bytes % 16) return FB_ERR_ARG;
+  if (s->n_seq < 1 || n < 0 || (n > 0 && (!src || !dst)) || n_layer < 1 || n_layer > 65535 || layer_bytes < 0 || layer_bytes % 16) return FB_ERR_ARG;
   const int64_t slots = (int64_t)s->table_ld * kPage;
   for (int i = 0; i < n; i++)
     if (src[i] < 0 || dst[i] < 0 || src[i] >= slots || dst[i] >= slots) return FB_ERR_RANGE;

@@ -89,3 +89,10 @@ def test_rows_that_cannot_be():
 def test_a_cache_needs_a_gpu():
     with pytest.raises(ValueError):
         kv4.KvCache4(1, 4, 2, 64, torch.zeros(1, 4, dtype=torch.int32))
+
+
+def test_moves_need_a_sequence():
+    lib = _lib.load()
+    none, one = _seqs(n_seq=0, n_tokens=0), (ctypes.c_int32 * 1)(3)
+    assert lib.fb_kv4_compact(ctypes.byref(none), 1, 0, 4096, 1, None) == _lib.FB_ERR_ARG
+    assert lib.fb_kv4_move(ctypes.byref(none), 1, 0, one, one, 1, None) == _lib.FB_ERR_ARG
