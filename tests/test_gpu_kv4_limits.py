@@ -347,3 +347,18 @@ def test_scratch_of_an_engine_goes_by_its_cache():
     torch.cuda.synchronize()
     eng.check()
     assert torch.equal(out, want)
+
+
+def test_a_prompt_of_several_chunks():
+    """More tokens than a pass takes: the bits of the passes one by one, and of the decode steps behind them."""
+    cfg = ModelArgs.from_name("tiny")
+    packed = packing.synth_packed(cfg, 0, device=DEV)
+    toks = torch.randint(0, cfg.vocab_size, (2300,), generator=torch.Generator().manual_seed(1), dtype=torch.int32).to(DEV)
+    whole, parts = (DecodeEngine(cfg, packed, max_seq=2400, kv_bits=4) for _ in range(2))
+    got, _ = whole.prefill(toks, 0)
+    cuts = [0, 766, 1533, 2300]
+    want = torch.cat([parts.prefill(toks[a:b], a)[0].clone() for a, b in zip(cuts, cuts[1:])])
+    assert torch.equal(got, want) and torch.equal(whole.cache.pool, parts.cache.pool)
+    assert torch.equal(whole.decode(5, 2300), parts.decode(5, 2300))
+    whole.check()
+    parts.check()
