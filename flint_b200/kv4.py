@@ -38,7 +38,7 @@ def page_bytes(n_kv: int, head_dim: int) -> int:
 
 
 class KvCache4:
-    """`table` int32 [n_seq, pages a sequence may have] on the GPU names the pages of every sequence; it stays the caller's, who may change its entries between
+    """`table` int32 [n_seq, pages a sequence may have], contiguous, on the GPU names the pages of every sequence; it stays the caller's, who may change its entries between
     calls. `pool` uint8 [n_layer, n_pages, n_kv, page bytes / n_kv] is allocated (zeroed) unless given. `rope_base` None: keys and queries come rotated."""
 
     def __init__(self, n_layer: int, n_pages: int, n_kv: int, head_dim: int, table: torch.Tensor, pool: Optional[torch.Tensor] = None,
@@ -49,8 +49,9 @@ class KvCache4:
         self.device = table.device
         if self.device.type != "cuda":
             raise ValueError(f"the page table must be on the GPU that runs the kernels, not on {self.device}")
-        if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1 or table.shape[1] < 1 or table.stride(0) < table.shape[1]:
-            raise ValueError("table must be int32 [n_seq, pages], its rows contiguous")
+        # rows side by side: the kernels hold a length on the GPU against what a row has room for, and a wider step from row to row would let it into the next one
+        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[1] < 1 or not table.is_contiguous():
+            raise ValueError("table must be contiguous int32 [n_seq, pages]")
         shape = (self.n_layer, self.n_pages, self.n_kv, record)
         if min(shape) < 1:
             raise ValueError(f"a pool of {shape} holds nothing")
@@ -64,7 +65,7 @@ class KvCache4:
         self._freq_ptr = _ptr(self.freq)
         self._status = torch.zeros(8, dtype=torch.int32, device=self.device)
         self._index = self.device.index if self.device.index is not None else torch.cuda.current_device()
-        self._ld = table.stride(0) if table.shape[0] > 1 else table.shape[1]
+        self._ld = table.shape[1]
         self._n_seq = table.shape[0]
         self._f32 = torch.empty(0, dtype=torch.float32, device=self.device)
         # what every call says about the cache; a call copies it and adds its own (a call costs the host microseconds, as much as a short kernel)

@@ -362,3 +362,21 @@ def test_a_prompt_of_several_chunks():
     assert torch.equal(whole.decode(5, 2300), parts.decode(5, 2300))
     whole.check()
     parts.check()
+
+
+def test_tables_whose_rows_are_apart_are_refused():
+    """A length on the GPU is held against the room of a row: with rows apart it could reach into the next one, or past the table."""
+    big = torch.arange(24, dtype=torch.int32, device=DEV).view(3, 8)
+    for table in (big[:, :4], big[:, 4:], big[::2], big.T, big.T[:, :2]):
+        with pytest.raises(ValueError):
+            KvCache4(1, 24, 2, 64, table)
+    c = KvCache4(1, 24, 2, 64, big[1:])
+    one = KvCache4(1, 24, 2, 64, big[2:, 4:])              # a piece of one row is a table
+    assert c.slots == 512 and one.slots == 256
+    x = rows(1, 2, 2, 64)
+    for cache, cached, start in ((c, ints(512, 511), ints(0, 1, 2)), (one, ints(255), None)):
+        before = cache.pool.clone()
+        cache.append(0, x, x, cached, start=start)
+        assert cache.status()["where"] == 22
+        written = (cache.pool != before).any(-1).any(-1).nonzero()[:, 1].tolist()
+        assert written == ([23] if cache is c else [])
